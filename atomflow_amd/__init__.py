@@ -32,6 +32,8 @@ AF_ERR_TIMEOUT = -10
 AF_KV_FP16 = 1
 AF_KV_FP8_E4M3 = 3
 AF_KV_POOL_SHARED_BLOCKS = 1
+AF_FP32 = 0
+AF_FP16 = 1
 
 
 class AfError(RuntimeError):

@@ -259,6 +259,42 @@ void launch_paged_qkv_rope_append(const __half* x, int64_t x_stride, int m, cons
           "launch_paged_qkv_rope_append");
 }
 
+void launch_quantize_rows(const __half* x, int64_t x_stride, int m, int n, int8_t* codes,
+                          int64_t codes_stride, float* scales, hipStream_t stream) {
+    check(af_quantize_rows(x, x_stride, m, n, codes, codes_stride, scales, stream),
+          "launch_quantize_rows");
+}
+
+void launch_silu_mul_quantize(const __half* gate, const __half* up, int64_t stride, int m, int n,
+                              int8_t* codes, int64_t codes_stride, float* scales,
+                              hipStream_t stream) {
+    check(af_silu_mul_quantize(gate, up, stride, m, n, codes, codes_stride, scales, stream),
+          "launch_silu_mul_quantize");
+}
+
+void launch_rmsnorm_quantize(const __half* x, int64_t x_stride, View& residual, const View& weight,
+                             float eps, int8_t* codes, int64_t codes_stride, float* scales,
+                             hipStream_t stream) {
+    if (residual.num_dims != 2 || weight.dtype != DataType::FP32)
+        throw std::runtime_error("launch_rmsnorm_quantize: residual [m, n], weight FP32 [n]");
+    check(af_rmsnorm_quantize(x, x_stride, residual.data_ptr, residual.data_ptr,
+                              residual.strides[0], int(residual.dtype),
+                              static_cast<const float*>(weight.data_ptr), eps,
+                              int(residual.dims[0]), int(residual.dims[1]), codes, codes_stride,
+                              scales, nullptr, 0, stream),
+          "launch_rmsnorm_quantize");
+}
+
+void launch_w8a8_gemm(const int8_t* x, int64_t x_stride, const float* x_scales,
+                      const int8_t* weight, int64_t w_stride, const float* w_scales,
+                      const float* bias, View& output, int k, hipStream_t stream) {
+    if (output.num_dims != 2) throw std::runtime_error("launch_w8a8_gemm: output [m, n]");
+    check(af_w8a8_gemm(x, x_stride, x_scales, int(output.dims[0]), weight, w_stride, w_scales, bias,
+                       output.data_ptr, output.strides[0], int(output.dtype), int(output.dims[1]), k,
+                       stream),
+          "launch_w8a8_gemm");
+}
+
 ArenaAllocator::ArenaAllocator(size_t total_size) {
     capacity_ = align_to_128(total_size);
     offset_ = 0;

@@ -11,7 +11,7 @@ import ctypes
 
 import numpy as np
 
-from . import AF_KV_FP16, AF_KV_FP8_E4M3, AfError, _abi, check, lib
+from . import AF_FP16, AF_KV_FP16, AF_KV_FP8_E4M3, AfError, _abi, check, lib
 from .device import DeviceBuffer, _s
 
 
@@ -96,6 +96,39 @@ def launch_qkv_rope_append(x, w_qkv, scales, k, qkv_out, k_cache, v_cache, cos_t
 
 
 # ---- prefill (multi-token append, causal attention over a prompt chunk) -----
+# ---- 8-bit integer projections -------------------------------------------------
+def launch_quantize_rows(x, x_stride, m, n, codes, codes_stride, scales, stream=None):
+    """fp16 rows to int8 codes with one fp32 scale per row (scale = max |x| / 127)."""
+    check(lib().af_quantize_rows(_p(x), x_stride, m, n, _p(codes), codes_stride, _p(scales),
+                                 _s(stream)), "launch_quantize_rows")
+
+
+def launch_silu_mul_quantize(gate, up, stride, m, n, codes, codes_stride, scales, stream=None):
+    """silu(gate) * up (fp16 rows, `stride` elements apart) to int8 codes and row scales."""
+    check(lib().af_silu_mul_quantize(_p(gate), _p(up), stride, m, n, _p(codes), codes_stride,
+                                     _p(scales), _s(stream)), "launch_silu_mul_quantize")
+
+
+def launch_rmsnorm_quantize(x, x_stride, weight, eps, m, n, codes=None, codes_stride=0, scales=None,
+                            residual=None, residual_out=None, residual_stride=0,
+                            residual_dtype=AF_FP16, normed=None, normed_stride=0, stream=None):
+    """residual_out = x + residual, and its RMSNorm as int8 codes and row scales and / or as fp16
+    rows (normed). residual_out may be residual; without both, the norm of x."""
+    check(lib().af_rmsnorm_quantize(_p(x), x_stride, _p(residual), _p(residual_out),
+                                    residual_stride, residual_dtype, _p(weight), eps, m, n,
+                                    _p(codes), codes_stride, _p(scales), _p(normed), normed_stride,
+                                    _s(stream)), "launch_rmsnorm_quantize")
+
+
+def launch_w8a8_gemm(x, x_stride, x_scales, m, weight, w_stride, w_scales, y, y_stride, n, k,
+                     bias=None, y_dtype=AF_FP16, stream=None):
+    """y[i, j] = (x[i] . weight[j]) * x_scales[i] * w_scales[j] (+ bias[j]), int8 codes, exact
+    integer sums."""
+    check(lib().af_w8a8_gemm(_p(x), x_stride, _p(x_scales), m, _p(weight), w_stride, _p(w_scales),
+                             _p(bias), _p(y), y_stride, y_dtype, n, k, _s(stream)),
+          "launch_w8a8_gemm")
+
+
 def launch_prefill_rope_append(qkv_out, n, k_cache, v_cache, cos_table, sin_table, p0, max_seq,
                                n_q_heads, n_kv_heads, head_dim, d_p0=None, d_status=None,
                                stream=None):
@@ -655,6 +688,7 @@ __all__ = [
     "decode_share_segments", "default_splits", "fp8_quantize", "kv_copy_blocks", "launch_cached_attention",
     "launch_cached_attention_ex", "launch_decode_attention_fused", "launch_paged_attention",
     "launch_paged_decode_fused", "launch_paged_rope_append", "launch_qkv_rope_append",
+    "launch_quantize_rows", "launch_rmsnorm_quantize", "launch_silu_mul_quantize", "launch_w8a8_gemm",
     "launch_w8a16_gemv", "launch_prefill_rope_append", "launch_prefill_attention",
     "launch_tiled_attention_kernel", "launch_paged_prefill_attention", "Scheduler",
     "launch_paged_prefill_attention_batched", "prefill_tile_map",

@@ -373,6 +373,63 @@ int af_qkv_rope_append(const void* x, const uint8_t* w_qkv, const void* scales, 
                        int head_dim, int32_t* d_status, af_stream_t stream);
 
 /* ======================================================================== */
+/* b1'. 8-bit integer projections: int8 activations and weights              */
+/* ======================================================================== */
+/* Element types of outputs and residual streams (the values of DataType,
+ * include/core/view.h). */
+#define AF_FP32 0
+#define AF_FP16 1
+
+/* Rows of int8 codes with one fp32 scale each: element value = code * scale.
+ * For a row v: a = max |v|, scale = a / 127, code = v * 127 / a rounded to
+ * nearest even, so codes are within +-127. A row of zeros (or of magnitudes
+ * below 2^-100) gets codes 0 and scale 1. A row that holds a NaN or an infinity
+ * gets codes 0 and scale NaN: what is computed from it is NaN.
+ * codes: row i at codes + i * codes_stride (bytes past n of a row are left as
+ * they are), any alignment; scales: [m]. Every row is n elements, n <= 2^30.
+ *
+ * af_quantize_rows: v = x, fp16 rows x_stride elements apart (attention's
+ * output, before the output projection). */
+int af_quantize_rows(const void* x, int64_t x_stride, int m, int n, int8_t* codes,
+                     int64_t codes_stride, float* scales, af_stream_t stream);
+/* v = silu(gate) * up in fp32, silu(g) = g / (1 + e^-g): the MLP's activation
+ * (the reference's swiglu_kernel, swiglu.cu:12-26, without its fp16 rounding).
+ * gate and up: fp16 rows `stride` elements apart; a fused gate and up product of
+ * rows [gate | up] has up = gate + n, stride >= 2 n. */
+int af_silu_mul_quantize(const void* gate, const void* up, int64_t stride, int m, int n,
+                         int8_t* codes, int64_t codes_stride, float* scales, af_stream_t stream);
+/* RMSNorm with the residual's addition (the reference's residual_add.cu:11-34
+ * followed by rms_norm_kernel, rmsnorm.cu:9-70), in one pass:
+ *   s = x + residual (fp32);  residual_out = s in the residual's type;
+ *   v = s / sqrt(mean(s^2) + eps) * weight
+ * and v as codes (codes, scales) or as fp16 rows (normed), or both; either may be
+ * NULL, not both. The norm is of the unrounded fp32 sum s. residual NULL (and
+ * residual_out NULL): v is the norm of x. residual_dtype: AF_FP16 or AF_FP32
+ * (both residual pointers; rows residual_stride elements apart). residual_out
+ * may be residual itself; no other output may overlap an input. weight: fp32
+ * [n]; 0 < eps < infinity. A row whose sum of squares is not finite in fp32
+ * counts as one that holds a NaN (normed is NaN; residual_out is s). */
+int af_rmsnorm_quantize(const void* x, int64_t x_stride, const void* residual, void* residual_out,
+                        int64_t residual_stride, int residual_dtype, const float* weight, float eps,
+                        int m, int n, int8_t* codes, int64_t codes_stride, float* scales,
+                        void* normed, int64_t normed_stride, af_stream_t stream);
+
+/* The W8A8 projection of m tokens:
+ *   y[i, j] = (sum_k x[i, k] * weight[j, k]) * x_scales[i] * w_scales[j] (+ bias[j])
+ * x: int8 rows x_stride bytes apart, one fp32 scale per token (as the quantisers
+ * above write them); weight: int8 [n, k] rows w_stride bytes apart, one fp32
+ * scale per output channel; bias: fp32 [n] or NULL; y: rows y_stride elements
+ * apart, y_dtype AF_FP16 or AF_FP32. The sums are exact 32-bit integers
+ * (any codes, -128 among them), so a token's row has the same bits whatever
+ * launch it is in: m, n and the other tokens change nothing. k, x_stride and
+ * w_stride are multiples of 16, k <= 131056 (so no sum overflows), strides below
+ * 2^23, x and weight 16-byte aligned; m and n are free (up to 2^26 each, m n up
+ * to 2^36), as are y_stride >= n and y's alignment (its element's). */
+int af_w8a8_gemm(const int8_t* x, int64_t x_stride, const float* x_scales, int m,
+                 const int8_t* weight, int64_t w_stride, const float* w_scales, const float* bias,
+                 void* y, int64_t y_stride, int y_dtype, int n, int k, af_stream_t stream);
+
+/* ======================================================================== */
 /* b2. Prefill: multi-token append and causal attention over a prompt chunk */
 /* ======================================================================== */
 /* Multi-token form of af_rope_append: n rows of qkv_out ([n, (n_q_heads +

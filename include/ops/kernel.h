@@ -159,6 +159,23 @@ void launch_w8a16_gemv_pair(const View& act_x, const View& w0, const View& s0, V
 void launch_w8a16_gemm_batched(const __half* x, int64_t x_stride, int m, const View& weight,
                                const View& scales, __half* y, int64_t y_stride, int group_size,
                                hipStream_t stream);
+// The int8 projection path. Activations and weights are codes of the int8 type
+// (View has no enumerator for it: raw pointers), one fp32 scale per row.
+// af_quantize_rows, af_silu_mul_quantize: fp16 rows (silu(gate) * up) to codes.
+void launch_quantize_rows(const __half* x, int64_t x_stride, int m, int n, int8_t* codes,
+                          int64_t codes_stride, float* scales, hipStream_t stream);
+void launch_silu_mul_quantize(const __half* gate, const __half* up, int64_t stride, int m, int n,
+                              int8_t* codes, int64_t codes_stride, float* scales,
+                              hipStream_t stream);
+// af_rmsnorm_quantize: residual += x and its norm, as codes. residual [m, n] FP16 or
+// FP32 rows, updated in place; weight FP32 [n].
+void launch_rmsnorm_quantize(const __half* x, int64_t x_stride, View& residual, const View& weight,
+                             float eps, int8_t* codes, int64_t codes_stride, float* scales,
+                             hipStream_t stream);
+// af_w8a8_gemm: output [m, n] FP16 or FP32 rows; bias fp32 [n] or nullptr.
+void launch_w8a8_gemm(const int8_t* x, int64_t x_stride, const float* x_scales,
+                      const int8_t* weight, int64_t w_stride, const float* w_scales,
+                      const float* bias, View& output, int k, hipStream_t stream);
 void launch_paged_qkv_rope_append(const __half* x, int64_t x_stride, int m, const View& w_qkv,
                                   const View& scales, int group_size, __half* qkv_out,
                                   const af_kv_pool& pool, int layer, const int64_t* d_slots,
