@@ -92,12 +92,18 @@ __device__ __forceinline__ void store8(float* p, int e, int n, const float (&v)[
     }
 }
 
-// Codes of v: fma(v, inv, 1.5 * 2^23) rounds the exact product to a whole number, to
-// nearest even (the sum's last place is 1), and leaves it in the low byte.
+// Codes of v: v * inv is within 2^-23 of v * 127 / a; adding 1.5 * 2^23 rounds it to a whole
+// number, to nearest even (the sum's last place is 1), and leaves that in the low byte. The
+// product is rounded by itself, as written in the formula, so that a program that computes it
+// in fp32 gets the same codes.
 __device__ __forceinline__ void store_codes(int8_t* p, int e, int n, const float (&v)[8], float inv) {
+#pragma clang fp contract(off)
     uint32_t b[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) b[i] = __builtin_bit_cast(uint32_t, fmaf(v[i], inv, 12582912.0f));
+    for (int i = 0; i < 8; ++i) {
+        const float q = v[i] * inv;
+        b[i] = __builtin_bit_cast(uint32_t, q + 12582912.0f);
+    }
     if (e + 8 <= n) {
         u32x2_a1 w;
 #pragma unroll
@@ -318,12 +324,24 @@ void launch_rows(const RowArgs& a, hipStream_t s) {
     hipLaunchKernelGGL((rows_kernel<MODE, T, CH>), dim3(blocks), dim3(T < 256 ? 256 : T), 0, s, a);
 }
 
+// Threads per row and chunks per thread by the row's length, measured for 1 to 8192 rows on
+// MI355X (us, plain / gated / norm with an fp16 residual). A thread's one chunk is best while
+// a workgroup can hold the row so: 45 rows of 4096 on 512 threads 2.2 / 2.6 / 3.0, on 256 with
+// two chunks each 2.4 / 2.9 / 3.6; 8192 rows 21.4 / 31.7 / 44.2 and 21.0 / 35.6 / 48.4. Short
+// rows take a wave each, which needs no barrier: 8192 rows of 1024 8.2 / 13.1 / 15.1, on 256
+// threads 9.9 / 13.5 / 17.5. Above 4096, 1024 threads suit few rows (45 of 5120: 2.4 / 3.0 /
+// 3.7, on 512 threads 2.6 / 3.5 / 4.2), and many only where the row fills them (8192 of 8192:
+// 40.9 / 61.7 / 85.0 and 36.8 / 62.1 / 88.1; of 5120: 34.0 / 47.8 / 66.1 and 26.8 / 43.4 / 59.4).
+// 85.0 us are 5.5 TB/s, what a large copy reaches on this card (5.15) and more.
 template <int MODE>
 void launch_slice(const RowArgs& a, hipStream_t s) {
+    const bool few = a.m < 2 * device_compute_units();
     if (a.n <= 512) launch_rows<MODE, 64, 1>(a, s);
+    else if (a.n <= 1024) launch_rows<MODE, 64, 2>(a, s);
     else if (a.n <= 2048) launch_rows<MODE, 256, 1>(a, s);
-    else if (a.n <= 4096) launch_rows<MODE, 256, 2>(a, s);
-    else if (a.n <= 8192) launch_rows<MODE, 256, 4>(a, s);
+    else if (a.n <= 4096) launch_rows<MODE, 512, 1>(a, s);
+    else if (a.n <= 8192 && (few || (MODE != kPlain && a.n > 7168))) launch_rows<MODE, 1024, 1>(a, s);
+    else if (a.n <= 8192) launch_rows<MODE, 512, 2>(a, s);
     else if (a.n <= 16384) launch_rows<MODE, 1024, 2>(a, s);
     else if (a.n <= 32768) launch_rows<MODE, 1024, 4>(a, s);
     else hipLaunchKernelGGL((long_rows_kernel<MODE>), dim3(unsigned(a.m)), dim3(1024), 0, s, a);
