@@ -168,8 +168,8 @@ class Graph:
 
 
 def _s(stream):
-    if stream is None:
-        return None
+    if stream is None or type(stream) is int:
+        return stream
     return stream.handle if isinstance(stream, Stream) else stream
 
 

@@ -16,8 +16,8 @@ from .device import DeviceBuffer, _s
 
 
 def _p(x):
-    if x is None:
-        return None
+    if x is None or type(x) is int:
+        return x
     return x.ptr if isinstance(x, DeviceBuffer) else int(x)
 
 
