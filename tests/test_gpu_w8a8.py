@@ -242,6 +242,48 @@ def test_w8a8_gemm(gpu, m, n, k, dtype, bias, pad):
     assert np.all(err <= gemm_bound(p, y, dtype)), (err - gemm_bound(p, y, dtype)).max()
 
 
+# Every form of the product, by its rule on a device of 256 CUs: one token in pairs of rows, the
+# tiles in the order of the table, with partial steps and tiles; for 256 x 256 tiles launches
+# of 1 to 13 steps, whole and partial, with one tile for some workgroups and two for others.
+FORMS = [(1, 4100, 14352), (1, 33, 4112), (1, 37, 131056), (2, 54, 14352), (17, 4211, 1024),
+         (18, 4121, 14352), (2, 8210, 128), (18, 8225, 1040), (17, 8457, 400), (4395, 65, 400),
+         (33, 4362, 14352), (68, 11231, 48), (66, 11037, 144), (34, 11531, 1040), (98, 4259, 528),
+         (34, 8311, 1040), (100, 8560, 1552), (67, 8462, 14352), (130, 11086, 1552),
+         (139, 11121, 2080), (135, 11085, 16), (129, 11300, 400), (4679, 385, 208),
+         (268, 10968, 1552), (539, 10659, 528), (515, 13437, 48), (525, 13664, 400),
+         (654, 10891, 528), (259, 10973, 48), (272, 10981, 400), (385, 11597, 1040)]
+WIDE = [(986, 11095, 16), (769, 13875, 48), (981, 10949, 128), (812, 13272, 144), (965, 11011, 256),
+        (965, 10859, 384), (806, 13146, 400), (777, 13348, 528), (1001, 10996, 1552),
+        (1931, 12351, 16), (2336, 10253, 48), (2187, 10909, 128), (2182, 11239, 144),
+        (2711, 8926, 256), (5279, 4618, 384), (3607, 6663, 400), (3090, 7818, 528),
+        (5006, 4896, 1040)]
+
+
+def check_product(m, n, k, dtype, bias, pad):
+    x, xs, w, ws, b = product_case(m, n, k, m + n + k)
+    b = b if bias else None
+    got = product_gpu(x, xs, w, ws, b, dtype, 48 * pad, 16 * pad, 3 * pad, pad)
+    assert np.isfinite(got).all()
+    for lo in range(0, m, 512):  # (bounds the host's arrays)
+        part = slice(lo, lo + 512)
+        _, p, y = gemm_parts(x[part], xs[part], w, ws, b)
+        over = np.abs(got[part].astype(np.float64) - y) - gemm_bound(p, y, dtype)
+        assert over.max() <= 0, (lo, over.max())
+
+
+@pytest.mark.parametrize("m,n,k", FORMS)
+@pytest.mark.parametrize("dtype,bias,pad", [(np.float16, True, 1), (np.float32, False, 0)])
+def test_w8a8_gemm_forms(gpu, m, n, k, dtype, bias, pad):
+    say(f"w8a8 form m={m} n={n} k={k} {np.dtype(dtype).name}")
+    check_product(m, n, k, dtype, bias, pad)
+
+
+@pytest.mark.parametrize("m,n,k", WIDE)
+def test_w8a8_gemm_wide(gpu, m, n, k):
+    say(f"w8a8 wide m={m} n={n} k={k}")
+    check_product(m, n, k, np.float32 if k % 32 else np.float16, n % 2 == 1, m % 2)
+
+
 @pytest.mark.parametrize("m,n", [(1, 1), (20, 3), (70, 40), (300, 129)])
 def test_w8a8_gemm_largest_sums(gpu, m, n):
     """The longest k with every code -128: 2^14 * 131056 just fits 32 bits."""
@@ -268,6 +310,19 @@ def test_w8a8_bits_do_not_depend_on_the_launch(gpu, n, k, dtype):
         rows = slice(n // 3, n // 3 + 40)
         part = product_gpu(x[lo:lo + m], xs[lo:lo + m], w[rows], ws[rows], b[rows], dtype)
         assert part.tobytes() == np.ascontiguousarray(whole[lo:lo + m, rows]).tobytes(), (lo, m)
+
+
+@pytest.mark.parametrize("m,n,k", [(2336, 10253, 48), (1001, 10996, 1552), (525, 13664, 400)])
+def test_w8a8_bits_of_large_launches(gpu, m, n, k):
+    """A large launch's rows and columns against small launches of some of them."""
+    say(f"w8a8 bits of a large launch m={m} n={n} k={k}")
+    x, xs, w, ws, b = product_case(m, n, k, n)
+    whole = product_gpu(x, xs, w, ws, b)
+    for lo, rows in ((0, 1), (255, 3), (m - 40, 40), (m // 2, 200)):
+        for c0, cols in ((0, 70), (250, 300), (n - 33, 33)):
+            t, j = slice(lo, lo + rows), slice(c0, c0 + cols)
+            part = product_gpu(x[t], xs[t], w[j], ws[j], b[j])
+            assert part.tobytes() == np.ascontiguousarray(whole[t, j]).tobytes(), (lo, c0)
 
 
 @pytest.mark.parametrize("m", [1, 40, 100, 300])
