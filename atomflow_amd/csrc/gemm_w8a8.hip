@@ -248,9 +248,15 @@ w8a8_tiled_kernel(const W8A8Args a) {
                       uint32_t(a.w_stride) + 16u * chunk(wave * WI + i);
     const uint32_t lds0 = lds_address(s_lds) + ks * L::kPart;
     const int steps = (a.k + KS * BK - 1) / (KS * BK);
+    // Workgroups that stream weights of their own begin at different steps: side by side at one
+    // k they would ask the same few memory channels for rows a power of two apart, and miss x
+    // together (45 x 28672 x 4096: 24.5 to 23.2 us, 32 x 128256 x 4096 89.8 to 87.4). The others
+    // share each step's operands in L2 (513 x 4096 x 14336 on 128 x 64 tiles: 83, turned 93).
+    const int turn = a.stream_w ? int(__umulhi(uint32_t(n0 / BN) * 2654435769u, uint32_t(steps))) : 0;
     auto issue = [&](int step, int buf) __attribute__((always_inline)) {
         const uint32_t dst = lds0 + buf * L::kStage;
-        const int k0 = (step * KS + ks) * BK;
+        const int turned = step + turn;
+        const int k0 = ((turned >= steps ? turned - steps : turned) * KS + ks) * BK;
         const char* xs = xb + k0;
         const char* ws = wb + k0;
         if (k0 + BK <= a.k) {
@@ -731,7 +737,7 @@ void launch_wide(const W8A8Args& a, hipStream_t s) {
 }
 
 // The forms (token rows, weight rows, parts of K, workgroups per CU), and what a launch of
-// each was measured to cost on MI355X (ten (n, k) shapes from 1024 x 1024 to 28672 x 4096, 2
+// each was measured to cost on MI355X (eleven (n, k) shapes from 1024 x 1024 to 128256 x 4096, 2
 // to 4096 tokens, weights read from HBM): a round of workgroups, `wgs` of them per CU while
 // tiles last, takes `round` plus per step (128 k of each part) `step`, for each workgroup of
 // the busiest CUs `share` and of the average CU `spread` (us); a launch `fixed` besides, and
@@ -743,25 +749,25 @@ struct TileCost {
     float fixed, round, step, share, spread, stream;
 };
 enum {
-    k16x16k8, k16x32k4, k32x32k4, k32x64k2, k64x32k4, k64x64, k64x64k2,
-    k128x64k2, k128x96, k128x128, k192x128, k256x256, k192x256, k128x128x2,
+    k16x16k8, k16x32k4, k32x32k4, k32x64k2, k64x32k4, k64x64k2, k128x64k2,
+    k128x96, k128x128, k192x128, k256x256, k192x256, k64x128, k128x128x2,
     kForms
 };
 constexpr TileCost kTileCost[kForms] = {
-    {16, 16, 8, 1, 1.5783f, 1.2261f, 0.2290f, 0.0f, 0.2208f, 0.0509f},
-    {16, 32, 4, 2, 1.8982f, 0.9154f, 0.0018f, 0.2466f, 0.0492f, 0.0805f},
-    {32, 32, 4, 1, 1.5663f, 1.6840f, 0.2953f, 0.0f, 0.1795f, 0.0482f},
-    {32, 64, 2, 2, 1.9182f, 0.9544f, 0.0777f, 0.2504f, 0.0594f, 0.0711f},
-    {64, 32, 4, 1, 1.5602f, 1.7892f, 0.5172f, 0.0f, 0.1125f, 0.0701f},
-    {64, 64, 1, 2, 1.4965f, 1.9512f, 0.0632f, 0.1714f, 0.0185f, 0.0634f},
-    {64, 64, 2, 1, 1.2712f, 2.0675f, 0.3872f, 0.0f, 0.0827f, 0.0733f},
-    {128, 64, 2, 1, 1.8047f, 2.7564f, 0.5192f, 0.0f, 0.2291f, 0.0570f},
-    {128, 96, 1, 1, 1.5140f, 3.7451f, 0.4027f, 0.0f, 0.0824f, 0.0381f},
-    {128, 128, 1, 1, 1.4138f, 2.9962f, 0.4100f, 0.0f, 0.1754f, 0.0557f},
-    {192, 128, 1, 1, 1.9038f, 4.2131f, 0.4738f, 0.0f, 0.3138f, 0.0243f},
-    {256, 256, 1, 1, 0.7078f, 7.7987f, 0.9615f, 0.0f, 0.5696f, 0.0545f},
-    {192, 256, 1, 1, 2.1838f, 5.9487f, 0.9013f, 0.0f, 0.4385f, 0.0375f},
-    {128, 128, 1, 2, 1.1181f, 3.8823f, 0.5302f, 0.0391f, 0.2155f, 0.0649f}
+    {16, 16, 8, 1, 1.7120f, 1.1334f, 0.2359f, 0.0f, 0.2412f, 0.0435f},
+    {16, 32, 4, 2, 2.1473f, 0.7189f, 0.0231f, 0.2282f, 0.0638f, 0.0730f},
+    {32, 32, 4, 1, 1.7303f, 1.5279f, 0.3059f, 0.0f, 0.1797f, 0.0421f},
+    {32, 64, 2, 2, 1.9726f, 0.9416f, 0.1054f, 0.2219f, 0.0798f, 0.0592f},
+    {64, 32, 4, 1, 1.3493f, 2.0178f, 0.5190f, 0.0f, 0.0958f, 0.0739f},
+    {64, 64, 2, 1, 1.3464f, 2.1042f, 0.4067f, 0.0f, 0.0729f, 0.0572f},
+    {128, 64, 2, 1, 1.8117f, 2.6802f, 0.5523f, 0.0f, 0.1929f, 0.0425f},
+    {128, 96, 1, 1, 1.7855f, 3.5270f, 0.3845f, 0.0f, 0.0958f, 0.0345f},
+    {128, 128, 1, 1, 1.4190f, 2.9689f, 0.4229f, 0.0f, 0.1518f, 0.0494f},
+    {192, 128, 1, 1, 1.6542f, 4.3061f, 0.4765f, 0.0f, 0.2935f, 0.0317f},
+    {256, 256, 1, 1, 0.8484f, 7.4613f, 0.9766f, 0.0f, 0.5346f, 0.0563f},
+    {192, 256, 1, 1, 2.1602f, 5.8443f, 0.8915f, 0.0f, 0.4288f, 0.0438f},
+    {64, 128, 1, 2, 2.5805f, 1.7073f, 0.1050f, 0.1910f, 0.1032f, 0.0660f},
+    {128, 128, 1, 2, 0.9998f, 3.9925f, 0.5376f, 0.0343f, 0.2072f, 0.0570f}
 };
 
 int pick_form(const W8A8Args& a) {
@@ -798,7 +804,6 @@ void launch_w8a8(const W8A8Args& a, hipStream_t s) {
         case k32x32k4: return launch_tiled<Y, 32, 32, 32, 1, 1, 4, 128, 4, 1>(a, s);
         case k32x64k2: return launch_tiled<Y, 32, 32, 64, 1, 2, 2, 128, 3, 2>(a, s);
         case k64x32k4: return launch_tiled<Y, 32, 64, 32, 2, 1, 4, 128, 3, 1>(a, s);
-        case k64x64: return launch_tiled<Y, 32, 64, 64, 2, 2, 1, 128, 4, 2>(a, s);
         case k64x64k2: return launch_tiled<Y, 32, 64, 64, 2, 2, 2, 128, 4, 1>(a, s);
         case k128x64k2: return launch_tiled<Y, 32, 128, 64, 2, 2, 2, 128, 3, 1>(a, s);
         case k128x96: return launch_tiled<Y, 32, 128, 96, 4, 1, 1, 128, 4, 1>(a, s);
@@ -806,6 +811,7 @@ void launch_w8a8(const W8A8Args& a, hipStream_t s) {
         case k192x128: return launch_tiled<Y, 32, 192, 128, 2, 4, 1, 128, 3, 1>(a, s);
         case k256x256: return launch_wide<Y>(a, s);
         case k192x256: return launch_tiled<Y, 32, 192, 256, 2, 4, 1, 128, 2, 1>(a, s);
+        case k64x128: return launch_tiled<Y, 32, 64, 128, 2, 2, 1, 128, 3, 2>(a, s);
         case k128x128x2: return launch_tiled<Y, 32, 128, 128, 2, 2, 1, 128, 2, 2>(a, s);
     }
 }

@@ -245,17 +245,18 @@ def test_w8a8_gemm(gpu, m, n, k, dtype, bias, pad):
 # Every form of the product, by its rule on a device of 256 CUs: one token in pairs of rows, the
 # tiles in the order of the table, with partial steps and tiles; for 256 x 256 tiles launches
 # of 1 to 13 steps, whole and partial, with one tile for some workgroups and two for others.
-FORMS = [(1, 4100, 14352), (1, 33, 4112), (1, 37, 131056), (2, 54, 14352), (17, 4211, 1024),
-         (18, 4121, 14352), (2, 8210, 128), (18, 8225, 1040), (17, 8457, 400), (4395, 65, 400),
-         (33, 4362, 14352), (68, 11231, 48), (66, 11037, 144), (34, 11531, 1040), (98, 4259, 528),
-         (34, 8311, 1040), (100, 8560, 1552), (67, 8462, 14352), (130, 11086, 1552),
-         (139, 11121, 2080), (135, 11085, 16), (129, 11300, 400), (4679, 385, 208),
-         (268, 10968, 1552), (539, 10659, 528), (515, 13437, 48), (525, 13664, 400),
-         (654, 10891, 528), (259, 10973, 48), (272, 10981, 400), (385, 11597, 1040)]
-WIDE = [(986, 11095, 16), (769, 13875, 48), (981, 10949, 128), (812, 13272, 144), (965, 11011, 256),
+FORMS = [(1, 4100, 14352), (1, 33, 4112), (1, 37, 131056), (2, 54, 14352), (33, 4362, 14352),
+         (17, 4211, 1024), (18, 4121, 14352), (2, 8210, 128), (18, 8225, 1040), (17, 8457, 400),
+         (4395, 65, 400), (33, 5193, 14352), (98, 4259, 528), (34, 8311, 1040), (100, 8560, 1552),
+         (67, 8462, 14352), (130, 11086, 1552), (139, 11121, 2080), (129, 11300, 400),
+         (4679, 385, 208), (196, 8792, 48), (539, 10659, 528), (266, 13342, 1552),
+         (515, 14499, 48), (525, 14634, 144), (586, 13115, 400), (513, 14851, 528),
+         (67, 10881, 16), (69, 11088, 400), (4131, 201, 1552), (65, 11432, 1040),
+         (259, 13824, 16), (325, 10899, 48), (261, 13611, 400), (385, 11597, 1040)]
+WIDE = [(986, 11095, 16), (991, 10899, 48), (981, 10949, 128), (812, 13272, 144), (965, 11011, 256),
         (965, 10859, 384), (806, 13146, 400), (777, 13348, 528), (1001, 10996, 1552),
-        (1931, 12351, 16), (2336, 10253, 48), (2187, 10909, 128), (2182, 11239, 144),
-        (2711, 8926, 256), (5279, 4618, 384), (3607, 6663, 400), (3090, 7818, 528),
+        (3670, 6695, 16), (1818, 13482, 48), (3588, 6882, 128), (2182, 11239, 144),
+        (1679, 14555, 256), (5279, 4618, 384), (3607, 6663, 400), (3090, 7818, 528),
         (5006, 4896, 1040)]
 
 
@@ -312,7 +313,7 @@ def test_w8a8_bits_do_not_depend_on_the_launch(gpu, n, k, dtype):
         assert part.tobytes() == np.ascontiguousarray(whole[lo:lo + m, rows]).tobytes(), (lo, m)
 
 
-@pytest.mark.parametrize("m,n,k", [(2336, 10253, 48), (1001, 10996, 1552), (525, 13664, 400)])
+@pytest.mark.parametrize("m,n,k", [(1818, 13482, 48), (1001, 10996, 1552), (586, 13115, 400)])
 def test_w8a8_bits_of_large_launches(gpu, m, n, k):
     """A large launch's rows and columns against small launches of some of them."""
     say(f"w8a8 bits of a large launch m={m} n={n} k={k}")
