@@ -839,7 +839,7 @@ extern "C" int af_w8a8_gemm(const int8_t* x, int64_t x_stride, const float* x_sc
         !aligned(bias, 4) || !aligned(y, y_dtype == AF_FP32 ? 4 : 2))
         return AF_ERR_INVALID_ARG;
     // a launch has fewer than 2^32 threads
-    if (m > 1 << 26 || n > 1 << 26 || int64_t(m) * n > int64_t(1) << 36) return AF_ERR_UNSUPPORTED;
+    if (m > 1 << 25 || n > 1 << 25 || int64_t(m) * n > int64_t(1) << 36) return AF_ERR_UNSUPPORTED;
     if (m == 0) return AF_OK;
     W8A8Args a{};
     a.x = x;

@@ -69,6 +69,24 @@ def quantize_fp8(w, group_size=128):
     return e4m3_codes(q).reshape(n, k), scale.astype(np.float16)
 
 
+def quantize_int8(w):
+    """[N, K] float -> (codes int8 [N, K], fp32 scales [N]), one scale per output channel: the
+    weights of ``kv.launch_w8a8_gemm``. scale = absmax / 127 (1 for a row of zeros, or of
+    magnitudes below 2^-100), codes = w * 127 / absmax rounded to nearest even, the rule of
+    the activations' quantisers. K is padded with zeros to whole 16 bytes, as the product
+    reads rows. Raises ValueError for values that are not finite."""
+    t = np.asarray(w, np.float32)
+    if t.ndim != 2:
+        raise ValueError(f"weights are [N, K], got {t.shape}")
+    if not np.isfinite(t).all():
+        raise ValueError("weights hold values that are not finite")
+    top = np.abs(t).max(axis=1, initial=0.0).astype(np.float64)
+    zero = top < 2.0 ** -100
+    codes = np.zeros((t.shape[0], -(-t.shape[1] // 16) * 16), np.int8)
+    codes[:, :t.shape[1]] = np.rint(np.where(zero, 0.0, 127.0 / np.where(zero, 1.0, top))[:, None] * t)
+    return codes, np.where(zero, 1.0, top / 127.0).astype(np.float32)
+
+
 def _pad(f):
     r = f.tell() % ALIGN
     if r:
@@ -172,4 +190,4 @@ class WeightFile:
 
 
 __all__ = ["AfError", "WeightFile", "e4m3_codes", "export_bin", "header_bytes", "layout_bytes",
-           "quantize_fp8"]
+           "quantize_fp8", "quantize_int8"]

@@ -423,7 +423,7 @@ int af_rmsnorm_quantize(const void* x, int64_t x_stride, const void* residual, v
  * (any codes, -128 among them), so a token's row has the same bits whatever
  * launch it is in: m, n and the other tokens change nothing. k, x_stride and
  * w_stride are multiples of 16, k <= 131056 (so no sum overflows), strides below
- * 2^23, x and weight 16-byte aligned; m and n are free (up to 2^26 each, m n up
+ * 2^23, x and weight 16-byte aligned; m and n are free (up to 2^25 each, m n up
  * to 2^36), as are y_stride >= n and y's alignment (its element's). */
 int af_w8a8_gemm(const int8_t* x, int64_t x_stride, const float* x_scales, int m,
                  const int8_t* weight, int64_t w_stride, const float* w_scales, const float* bias,

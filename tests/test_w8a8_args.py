@@ -1,8 +1,14 @@
 """Refusals of the int8 projection path, all before any device call: the pointers are
 never dereferenced."""
+import os
+import subprocess
+
+import numpy as np
 import pytest
 
 import atomflow_amd
+import w8a8_ref
+from atomflow_amd import weights
 from atomflow_amd import (AF_ERR_INVALID_ARG, AF_ERR_UNSUPPORTED, AF_FP16, AF_FP32, AF_KV_FP8_E4M3, AF_OK,
                           kv)
 
@@ -36,8 +42,8 @@ BAD, NOT = AF_ERR_INVALID_ARG, AF_ERR_UNSUPPORTED
     (dict(w_stride=1 << 23), NOT), (dict(x=FAKE + 8), BAD), (dict(w=FAKE + 1), BAD),
     (dict(xs=FAKE + 2), BAD), (dict(ws=FAKE + 2), BAD), (dict(bias=FAKE + 2), BAD),
     (dict(y=FAKE + 1), BAD), (dict(y=FAKE + 2, y_dtype=AF_FP32), BAD), (dict(y_dtype=2), NOT),
-    (dict(y_dtype=AF_KV_FP8_E4M3), NOT), (dict(m=(1 << 26) + 1), NOT),
-    (dict(n=(1 << 26) + 1, y_stride=1 << 27), NOT),
+    (dict(y_dtype=AF_KV_FP8_E4M3), NOT), (dict(m=(1 << 25) + 1), NOT),
+    (dict(n=(1 << 25) + 1, y_stride=1 << 27), NOT),
     (dict(m=1 << 20, n=1 << 17, y_stride=1 << 17), NOT), (dict(m=0), AF_OK)])
 def test_w8a8_gemm_refusals(changes, status):
     assert call("af_w8a8_gemm", GEMM, **changes) == status
@@ -87,3 +93,74 @@ def test_python_mirror_raises():
         kv.launch_quantize_rows(FAKE, 4, 1, 8, FAKE, 8, FAKE)
     with pytest.raises(atomflow_amd.AfError):
         kv.launch_silu_mul_quantize(FAKE, None, 8, 1, 8, FAKE, 8, FAKE)
+
+
+def test_cpp_launchers_refuse(tmp_path):
+    """The C++ wrappers check their Views and throw with the status text; nothing reaches a device."""
+    src = tmp_path / "t.cpp"
+    src.write_text(r'''
+#include <cstdio>
+#include <functional>
+#include <stdexcept>
+#include <string>
+#include "ops/kernel.h"
+static int bad = 0;
+static void throws(const char* what, const char* text, const std::function<void()>& f) {
+    try { f(); } catch (const std::runtime_error& e) {
+        if (std::string(e.what()).find(text) == std::string::npos) { std::printf("%s: %s\n", what, e.what()); ++bad; }
+        return;
+    }
+    std::printf("%s did not throw\n", what);
+    ++bad;
+}
+int main() {
+    char* fake = reinterpret_cast<char*>(0x10000);
+    auto h = reinterpret_cast<__half*>(fake);
+    auto c = reinterpret_cast<int8_t*>(fake);
+    auto f = reinterpret_cast<float*>(fake);
+    View y = create_contiguous_view(fake, DataType::FP16, {4, 32});
+    View res = create_contiguous_view(fake, DataType::FP32, {4, 64});
+    View w = create_contiguous_view(fake, DataType::FP32, {64});
+    throws("gemm k", "unsupported", [&] { launch_w8a8_gemm(c, 48, f, c, 48, f, nullptr, y, 40, nullptr); });
+    throws("gemm x", "invalid", [&] { launch_w8a8_gemm(nullptr, 64, f, c, 64, f, nullptr, y, 64, nullptr); });
+    View y3 = create_contiguous_view(fake, DataType::FP16, {2, 2, 32});
+    throws("gemm dims", "output", [&] { launch_w8a8_gemm(c, 64, f, c, 64, f, nullptr, y3, 64, nullptr); });
+    View y8 = create_contiguous_view(fake, DataType::FP8_E4M3, {4, 32});
+    throws("gemm type", "unsupported", [&] { launch_w8a8_gemm(c, 64, f, c, 64, f, nullptr, y8, 64, nullptr); });
+    throws("norm eps", "invalid", [&] { launch_rmsnorm_quantize(h, 64, res, w, 0.0f, c, 64, f, nullptr); });
+    View wh = create_contiguous_view(fake, DataType::FP16, {64});
+    throws("norm weight", "weight", [&] { launch_rmsnorm_quantize(h, 64, res, wh, 1e-5f, c, 64, f, nullptr); });
+    View rb = create_contiguous_view(fake, DataType::BF16, {4, 64});
+    throws("norm residual", "unsupported", [&] { launch_rmsnorm_quantize(h, 64, rb, w, 1e-5f, c, 64, f, nullptr); });
+    throws("quantize", "invalid", [&] { launch_quantize_rows(h, 63, 4, 64, c, 64, f, nullptr); });
+    throws("silu", "invalid", [&] { launch_silu_mul_quantize(h, nullptr, 64, 4, 64, c, 64, f, nullptr); });
+    if (!bad) std::puts("ok");
+    return bad;
+}
+''')
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    lib = os.path.dirname(atomflow_amd.LIB_PATH)
+    exe = tmp_path / "t"
+    subprocess.run(["g++", "-std=c++17", "-O1", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include", "-I",
+                    os.path.join(root, "include"), str(src), "-L", lib, "-latomflow_kv",
+                    "-L/opt/rocm/lib", "-lamdhip64", f"-Wl,-rpath,{lib}:/opt/rocm/lib", "-o", str(exe)],
+                   check=True)
+    r = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert r.returncode == 0 and r.stdout.strip() == "ok", (r.stdout, r.stderr)
+
+
+@pytest.mark.parametrize("n,k", [(5, 64), (3, 100), (1, 1), (40, 4096)])
+def test_quantize_int8(n, k):
+    r = np.random.default_rng(n + k)
+    w = (r.standard_normal((n, k)) * r.uniform(1e-3, 3.0, (n, 1))).astype(np.float32)
+    w[n // 2] = 0.0
+    codes, scales = weights.quantize_int8(w)
+    assert codes.dtype == np.int8 and codes.shape == (n, -(-k // 16) * 16) and scales.dtype == np.float32
+    assert np.all(codes[:, k:] == 0)
+    w8a8_ref.assert_codes(codes[:, :k], scales, w.astype(np.float64), 0.0)
+
+
+def test_quantize_int8_refuses():
+    for bad in (np.zeros(4), np.full((2, 3), np.nan), np.array([[1.0, np.inf]])):
+        with pytest.raises(ValueError):
+            weights.quantize_int8(bad)
