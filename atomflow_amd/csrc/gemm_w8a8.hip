@@ -771,17 +771,20 @@ constexpr TileCost kTileCost[kForms] = {
 };
 
 int pick_form(const W8A8Args& a) {
-    const int64_t cus = device_compute_units();
+    // (called for every launch: constant tile sizes, 32-bit arithmetic; tiles are below 2^29)
+    const unsigned cus = unsigned(device_compute_units());
+    const unsigned m = unsigned(a.m), n = unsigned(a.n), k = unsigned(a.k);
     const float mb = float(a.n) * float(a.k) * 1e-6f;
     int best = 0;
     float best_cost = 0.0f;
+#pragma clang loop unroll(full)
     for (int i = 0; i < kForms; ++i) {
+        constexpr auto up = [](unsigned x, int by) { return (x + by - 1) / unsigned(by); };
         const TileCost& c = kTileCost[i];
-        const int64_t tiles = int64_t((a.m + c.bm - 1) / c.bm) * ((a.n + c.bn - 1) / c.bn);
-        const int64_t per_cu = (tiles + cus - 1) / cus;  // of the busiest CUs
-        const int64_t rounds = (per_cu + c.wgs - 1) / c.wgs;
-        const float steps = float((a.k + 128 * c.ks - 1) / (128 * c.ks));
-        const float cost = c.fixed + float(rounds) * (c.round + steps * c.step) +
+        const unsigned tiles = up(m, c.bm) * up(n, c.bn);
+        const unsigned per_cu = (tiles + cus - 1) / cus;  // of the busiest CUs
+        const float steps = float(up(k, 128 * c.ks));
+        const float cost = c.fixed + float(up(per_cu, c.wgs)) * (c.round + steps * c.step) +
                            steps * (float(per_cu) * c.share + float(tiles) / float(cus) * c.spread) +
                            mb * c.stream;
         if (i == 0 || cost < best_cost) {

@@ -13,6 +13,12 @@ void check(int status, const char* what) {
         throw std::runtime_error(std::string(what) + ": " + af_status_string(status));
 }
 
+// Rows of adjacent elements whose dims the C ABI's ints hold.
+bool is_matrix(const View& v) {
+    return v.num_dims == 2 && v.strides[1] == 1 && v.dims[0] >= 0 && v.dims[0] <= INT32_MAX &&
+           v.dims[1] >= 0 && v.dims[1] <= INT32_MAX;
+}
+
 }  // namespace
 
 void launch_rope(const View& q_input, const View& k_input, const float* cos_cache,
@@ -275,7 +281,8 @@ void launch_silu_mul_quantize(const __half* gate, const __half* up, int64_t stri
 void launch_rmsnorm_quantize(const __half* x, int64_t x_stride, View& residual, const View& weight,
                              float eps, int8_t* codes, int64_t codes_stride, float* scales,
                              hipStream_t stream) {
-    if (residual.num_dims != 2 || weight.dtype != DataType::FP32)
+    if (!is_matrix(residual) || weight.dtype != DataType::FP32 || weight.num_dims != 1 ||
+        weight.dims[0] != residual.dims[1] || weight.strides[0] != 1)
         throw std::runtime_error("launch_rmsnorm_quantize: residual [m, n], weight FP32 [n]");
     check(af_rmsnorm_quantize(x, x_stride, residual.data_ptr, residual.data_ptr,
                               residual.strides[0], int(residual.dtype),
@@ -288,7 +295,7 @@ void launch_rmsnorm_quantize(const __half* x, int64_t x_stride, View& residual, 
 void launch_w8a8_gemm(const int8_t* x, int64_t x_stride, const float* x_scales,
                       const int8_t* weight, int64_t w_stride, const float* w_scales,
                       const float* bias, View& output, int k, hipStream_t stream) {
-    if (output.num_dims != 2) throw std::runtime_error("launch_w8a8_gemm: output [m, n]");
+    if (!is_matrix(output)) throw std::runtime_error("launch_w8a8_gemm: output [m, n]");
     check(af_w8a8_gemm(x, x_stride, x_scales, int(output.dims[0]), weight, w_stride, w_scales, bias,
                        output.data_ptr, output.strides[0], int(output.dtype), int(output.dims[1]), k,
                        stream),

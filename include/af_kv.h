@@ -387,6 +387,7 @@ int af_qkv_rope_append(const void* x, const uint8_t* w_qkv, const void* scales, 
  * gets codes 0 and scale NaN: what is computed from it is NaN.
  * codes: row i at codes + i * codes_stride (bytes past n of a row are left as
  * they are), any alignment; scales: [m]. Every row is n elements, n <= 2^30.
+ * Outputs overlap no input and no other output unless said so.
  *
  * af_quantize_rows: v = x, fp16 rows x_stride elements apart (attention's
  * output, before the output projection). */
@@ -406,8 +407,7 @@ int af_silu_mul_quantize(const void* gate, const void* up, int64_t stride, int m
  * NULL, not both. The norm is of the unrounded fp32 sum s. residual NULL (and
  * residual_out NULL): v is the norm of x. residual_dtype: AF_FP16 or AF_FP32
  * (both residual pointers; rows residual_stride elements apart). residual_out
- * may be residual itself; no other output may overlap an input. weight: fp32
- * [n]; 0 < eps < infinity. A row whose sum of squares is not finite in fp32
+ * may be residual itself. weight: fp32 [n]; 0 < eps < infinity. A row whose sum of squares is not finite in fp32
  * counts as one that holds a NaN (normed is NaN; residual_out is s). */
 int af_rmsnorm_quantize(const void* x, int64_t x_stride, const void* residual, void* residual_out,
                         int64_t residual_stride, int residual_dtype, const float* weight, float eps,

@@ -197,6 +197,59 @@ def test_norm_of_rows_past_fp32_squares(gpu):
     assert np.array_equal(ro.get(), residual)
 
 
+def test_more_rows_than_one_launch(gpu):
+    """A launch takes 2^21 rows: the rows on both sides of its end, and the last."""
+    say("quantise and normalise 2^21 + 37 rows")
+    m, n = 2 ** 21 + 37, 24
+    r = np.random.default_rng(5)
+    x = (r.standard_normal((m, n), np.float32)).astype(np.float16)
+    w = np.ones(n, np.float32)
+    dx, c, s = up(x), Rows(np.int8, m, n, n), Rows(np.float32, m, 1, 1)
+    kv.launch_quantize_rows(dx, n, m, n, c.ptr, n, s.ptr)
+    assert_codes(c.get(), s.get()[:, 0], x.astype(np.float64), 0.0)
+    kv.launch_rmsnorm_quantize(dx, n, up(w), 1e-5, m, n, codes=c.ptr, codes_stride=n, scales=s.ptr)
+    _, v = rmsnorm(x, None, w, 1e-5)
+    assert_codes(c.get(), s.get()[:, 0], v, norm_delta(n))
+
+
+def put_rows(buf, a, stride):
+    """Rows of a, `stride` elements apart."""
+    for i, row in enumerate(a):
+        buf.upload(row, offset=i * stride * a.itemsize)
+
+
+def get_rows(buf, dtype, m, n, stride):
+    size = np.dtype(dtype).itemsize
+    return np.stack([buf.download(dtype, (n,), offset=i * stride * size) for i in range(m)])
+
+
+def test_row_offsets_past_32_bits(gpu):
+    say("rows whose offsets pass 2^32 elements")
+    m, n, far = 4, 300, (1 << 31) + 40
+    x, res = activations(m, n, 1), activations(m, n, 2)
+    w = np.ones(n, np.float32)
+    bufs = [dev.DeviceBuffer(2 * (far * (m - 1) + n)) for _ in range(4)]
+    dx, dr, dro, dn = bufs
+    c, s = dev.DeviceBuffer(far * (m - 1) + n), dev.DeviceBuffer(4 * m)
+    put_rows(dx, x, far)
+    put_rows(dr, res, far)
+    kv.launch_quantize_rows(dx, far, m, n, c, far, s)
+    assert_codes(get_rows(c, np.int8, m, n, far), s.download(np.float32), x.astype(np.float64), 0.0)
+    kv.launch_silu_mul_quantize(dx, dr, far, m, n, c, far, s)
+    assert_codes(get_rows(c, np.int8, m, n, far), s.download(np.float32), silu_mul(x, res), silu_delta(x))
+    kv.launch_rmsnorm_quantize(dx, far, up(w), 1e-5, m, n, codes=c, codes_stride=far, scales=s,
+                               residual=dr, residual_out=dro, residual_stride=far, normed=dn,
+                               normed_stride=far)
+    s64, v = rmsnorm(x, res, w, 1e-5)
+    assert_codes(get_rows(c, np.int8, m, n, far), s.download(np.float32), v, norm_delta(n))
+    assert np.array_equal(get_rows(dro, np.float16, m, n, far),
+                          (x.astype(np.float32) + res.astype(np.float32)).astype(np.float16))
+    normed = get_rows(dn, np.float16, m, n, far).astype(np.float64)
+    assert np.all(np.abs(normed - v) <= 1.01 * norm_delta(n) * np.abs(v) + 0.5 * fp16_ulp(v))
+    for b in bufs + [c]:
+        b.free()
+
+
 # ---- the product ----------------------------------------------------------------
 
 
@@ -343,6 +396,44 @@ def test_w8a8_odd_scales(gpu, m):
     assert np.array_equal(np.isinf(got), np.isinf(want))
     ok = np.isfinite(want)
     assert np.all(np.abs(got[ok] - want[ok]) <= fp16_ulp(want[ok]))
+
+
+@pytest.mark.parametrize("m", [1, 3, 40, 300])
+def test_w8a8_fp16_extremes(gpu, m):
+    """Subnormal, just overflowing and tied results: the bits of fp32 products rounded once."""
+    say(f"w8a8 fp16 extremes m={m}")
+    n, k = 400, 64
+    x, xs, w, _, _ = product_case(m, n, k, m)
+    ws = np.float32(2.0) ** np.random.default_rng(2).integers(-42, 14, n).astype(np.float32)
+    xs[:] = np.float32(2.0) ** -4
+    got = product_gpu(x, xs, w, ws)
+    acc = (x.astype(np.int32) @ w.astype(np.int32).T).astype(np.float32)
+    with np.errstate(over="ignore"):
+        want = (acc * xs[:, None] * ws).astype(np.float16)
+    assert np.isinf(want).any() and (np.abs(want[want != 0]) < 2.0 ** -14).any()
+    assert np.array_equal(got == 0, want == 0)
+    assert np.array_equal(np.where(got == 0, 0, got.view(np.uint16)),
+                          np.where(want == 0, 0, want.view(np.uint16)))
+
+
+@pytest.mark.parametrize("m,n,k", [(600, 70, 64), (520, 9000, 144)])
+def test_w8a8_offsets_past_32_bits(gpu, m, n, k):
+    """Rows of x, w and y whose byte offsets pass 2^32."""
+    say(f"w8a8 offsets past 32 bits m={m} n={n}")
+    xstr, ystr = (1 << 23) - 16, (1 << 22) + 3
+    wstr = xstr if n < 2 * m else (1 << 19) + 16
+    x, xs, w, ws, b = product_case(m, n, k, m)
+    dx, dw = dev.DeviceBuffer(xstr * (m - 1) + k), dev.DeviceBuffer(wstr * (n - 1) + k)
+    y = dev.DeviceBuffer(4 * (ystr * (m - 1) + n))
+    assert min(xstr * (m - 1), 4 * ystr * (m - 1)) > 2 ** 32
+    put_rows(dx, x, xstr)
+    put_rows(dw, w, wstr)
+    kv.launch_w8a8_gemm(dx, xstr, up(xs), m, dw, wstr, up(ws), y, ystr, n, k, bias=up(b), y_dtype=AF_FP32)
+    got = get_rows(y, np.float32, m, n, ystr)
+    _, p, want = gemm_parts(x, xs, w, ws, b)
+    assert np.all(np.abs(got - want) <= gemm_bound(p, want, np.float32))
+    for d in (dx, dw, y):
+        d.free()
 
 
 def test_codes_of_a_row_with_a_nan_make_its_products_nan(gpu):

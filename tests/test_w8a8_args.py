@@ -129,6 +129,13 @@ int main() {
     throws("gemm type", "unsupported", [&] { launch_w8a8_gemm(c, 64, f, c, 64, f, nullptr, y8, 64, nullptr); });
     throws("norm eps", "invalid", [&] { launch_rmsnorm_quantize(h, 64, res, w, 0.0f, c, 64, f, nullptr); });
     View wh = create_contiguous_view(fake, DataType::FP16, {64});
+    View ws = create_contiguous_view(fake, DataType::FP32, {63});
+    throws("norm length", "weight", [&] { launch_rmsnorm_quantize(h, 64, res, ws, 1e-5f, c, 64, f, nullptr); });
+    View far = create_contiguous_view(fake, DataType::FP16, {int64_t(1) << 32, 32});
+    throws("gemm rows", "output", [&] { launch_w8a8_gemm(c, 64, f, c, 64, f, nullptr, far, 64, nullptr); });
+    View tr = y;
+    tr.strides[1] = 2;
+    throws("gemm columns", "output", [&] { launch_w8a8_gemm(c, 64, f, c, 64, f, nullptr, tr, 64, nullptr); });
     throws("norm weight", "weight", [&] { launch_rmsnorm_quantize(h, 64, res, wh, 1e-5f, c, 64, f, nullptr); });
     View rb = create_contiguous_view(fake, DataType::BF16, {4, 64});
     throws("norm residual", "unsupported", [&] { launch_rmsnorm_quantize(h, 64, rb, w, 1e-5f, c, 64, f, nullptr); });
