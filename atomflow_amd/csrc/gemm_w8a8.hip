@@ -212,6 +212,7 @@ w8a8_tiled_kernel(const W8A8Args a) {
     static_assert(BK == 64 || BK == 128 || BK == 256, "the swizzles that are written down");
     static_assert(XI * kDmaRows * NW == BM && WI * kDmaRows * NW == BN, "uneven DMA");
     static_assert(MT >= 1 && NT >= 1 && ST >= 2, "tile too small for its waves");
+    static_assert(Q % 2 == 0, "the next step's first operands take the slot that its last leave");
     __shared__ __align__(16) char s_lds[L::kLds];
 
     const int lane = threadIdx.x & 63;
