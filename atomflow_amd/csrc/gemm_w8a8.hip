@@ -8,8 +8,9 @@
 // row does not depend on the launch it is in. The sum becomes fp32 (its one rounding
 // before the result's, 2^-25 relative at most) and takes the scales and the bias there.
 //
-// Two kernels: few tokens (w8a8_few_kernel), bound by the weights' stream, and tiles
-// (w8a8_tiled_kernel), bound by the matrix cores.
+// Three kernels: one token (w8a8_row_kernel) and the tiles of few tokens (w8a8_tiled_kernel)
+// are bound by the weights' stream, tiles in between by what a CU loads from L2, large
+// launches (w8a8_wide_kernel) by the card's power. pick_form chooses by measured cost.
 #include <algorithm>
 
 #include "af_common.h"
@@ -37,7 +38,7 @@ struct W8A8Args {
     void* y;              // fp16 (Y = uint16_t) or fp32 (float) rows, y_stride elements apart
     int64_t y_stride;
     int m, n, k;
-    int stream_w;         // non-temporal weight loads
+    int stream_w;         // each weight row is read by one workgroup: see launch_tiled
 };
 
 // What tail chunks past k load in place of codes.
@@ -58,7 +59,9 @@ __device__ __forceinline__ uint32_t half_pair(float lo, float hi) {
 // contiguous 1 KB chunks, 16 bytes per lane, non-temporally (each weight byte is read once
 // by the launch); a chunk of the token's codes is loaded once for the R rows. All loads of a
 // pass of U chunks go out before any is used. v_dot4_i32_i8 adds four products a lane, and
-// the lanes' sums meet by cross-lane adds.
+// the lanes' sums meet by cross-lane adds. Bound by HBM: 28672 x 4096 in 18.2 us, 128256 x
+// 4096 in 74, 7.1 TB/s (a 16 x 16 x 64 matrix-core product fed with 64-byte pieces of 16 rows
+// took 25.6 and 123). Two tokens are no faster here than on the tiles.
 constexpr int kRowWaves = 4;
 
 __device__ __forceinline__ int wave_sum_i32(int v) {
@@ -117,16 +120,26 @@ __global__ __launch_bounds__(64 * kRowWaves) void w8a8_row_kernel(const W8A8Args
 }
 
 // ---- tiles ----------------------------------------------------------------------
-// A workgroup of WR x WC waves makes a BM x BN tile of y (tokens x weight rows) in steps of
-// BK bytes of k; D = W X^T on v_mfma_i32_32x32x32_i8, so that a lane's registers run along
-// y's rows. A stage of LDS holds a step's BM + BN rows of BK bytes, fetched without registers
-// (16 bytes per lane, 1 KB per wave-instruction); ST stages. Rows past m or n load the last
-// row (not stored); chunks past k load zeros.
+// A workgroup of WR x WC waves for each of KS parts of K makes a BM x BN tile of y (tokens x
+// weight rows) in steps of 128 bytes of k per part; D = W X^T, so that a lane's registers run
+// along y's rows. A stage of LDS holds a step's BM + BN rows of 128 bytes (per part), fetched
+// without registers (16 bytes per lane, 8 rows per wave-instruction); ST stages. Rows past m
+// or n load the last row (not stored); chunks past k load zeros. The parts' sums meet in LDS.
 //
-// Operands are read one sub-step (32 of k) ahead of the products, over the step's end: when
-// a step's last operands are in registers and the next stage has arrived, one barrier both
-// publishes that stage and frees the one just read, whose place the step ST ahead takes; the
-// next stage's first operands are read under the last products of this one.
+// Operands are read one sub-step ahead of the products, over the step's end: when a step's
+// last operands are in registers and the next stage has arrived, one barrier both publishes
+// that stage and frees the one just read, whose place the step ST ahead takes; the next
+// stage's first operands are read under the last products of this one. A part of one wave
+// needs no barrier: it loads what it reads.
+//
+// What bounds it, between a few dozen and a few hundred tokens, is the loads: 8 rows of 128
+// bytes an instruction reach 98 GB/s per CU from L2 (1 KB pieces 145), and HBM's latency. 513
+// x 4096 x 14336 runs in 60 us with the matrix cores busy a quarter of the time; stages twice
+// as many or as long, operands a whole step ahead, and a wave that touches the weights' lines
+// early gave nothing or cost time.
+constexpr int kStep = 128;
+
+// lds_dma16 of a wave-uniform base and lane offsets, non-temporal.
 __device__ __forceinline__ void lds_dma16_nt(const void* base, uint32_t off, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(lds),
                  "v"(off), "s"(base)
@@ -155,19 +168,16 @@ struct Mfma<16> {
     }
 };
 
-template <int BK>
+// 16-byte chunk c of row r sits at chunk c ^ (r / 2 % 8): the 16 lanes of a 256-byte LDS
+// access of an operand read (16 rows, one chunk) cover all 64 banks. (With the pattern
+// repeating after 8 rows, half of the LDS's cycles were conflicts.)
 __device__ __forceinline__ uint32_t swizzled(int row, int chunk) {
-    // Chunk c of row r sits at chunk c ^ f(r): the 16 lanes of a 256-byte LDS access of an
-    // operand read (16 rows, one chunk) cover all 64 banks. (With f repeating after 8 rows,
-    // half of the LDS's cycles were conflicts.)
-    if constexpr (BK == 256) return uint32_t(chunk ^ (row & 15));
-    else if constexpr (BK == 128) return uint32_t(chunk ^ ((row >> 1) & 7));
-    else return uint32_t(chunk ^ ((row >> 2) & 3));
+    return uint32_t(chunk ^ ((row >> 1) & 7));
 }
 
-template <int kY, int S, int BM, int BN, int WR, int WC, int KS, int BK, int ST>
+template <int kY, int S, int BM, int BN, int WR, int WC, int KS, int ST>
 struct TileLds {
-    static constexpr int kPart = (BM + BN) * BK;     // a part of K's rows in a stage
+    static constexpr int kPart = (BM + BN) * kStep;     // a part of K's rows in a stage
     static constexpr int kStage = KS * kPart;
     static constexpr int kRows = S * WR;            // tokens of an output pass
     static constexpr int kOut = kRows * (kY * BN + 16);
@@ -199,17 +209,16 @@ __device__ __forceinline__ void store_pass(const W8A8Args& a, const char* s_out,
     }
 }
 
-template <typename Y, int S, int BM, int BN, int WR, int WC, int KS, int BK, int ST, int WGS>
+template <typename Y, int S, int BM, int BN, int WR, int WC, int KS, int ST, int WGS>
 __global__ __launch_bounds__(64 * WR * WC * KS, (WGS * WR * WC * KS + 3) / 4) void
 w8a8_tiled_kernel(const W8A8Args a) {
-    using L = TileLds<sizeof(Y), S, BM, BN, WR, WC, KS, BK, ST>;
+    using L = TileLds<sizeof(Y), S, BM, BN, WR, WC, KS, ST>;
     constexpr int NW = WR * WC, THREADS = 64 * NW * KS;
     constexpr int MT = BM / WR / S, NT = BN / WC / S;  // S x S tiles of a wave
     constexpr int C = Mfma<S>::kChunks, G = Mfma<S>::kGroups;
-    constexpr int kRowLanes = BK / 16, kDmaRows = 64 / kRowLanes;  // a DMA instruction's rows
+    constexpr int kRowLanes = kStep / 16, kDmaRows = 64 / kRowLanes;  // a DMA instruction's rows
     constexpr int XI = BM / kDmaRows / NW, WI = BN / kDmaRows / NW;
-    constexpr int Q = BK / 16 / C;  // sub-steps
-    static_assert(BK == 64 || BK == 128 || BK == 256, "the swizzles that are written down");
+    constexpr int Q = kStep / 16 / C;  // sub-steps
     static_assert(XI * kDmaRows * NW == BM && WI * kDmaRows * NW == BN, "uneven DMA");
     static_assert(MT >= 1 && NT >= 1 && ST >= 2, "tile too small for its waves");
     static_assert(Q % 2 == 0, "the next step's first operands take the slot that its last leave");
@@ -234,7 +243,7 @@ w8a8_tiled_kernel(const W8A8Args a) {
     // The chunk that the lane's place in DMA instruction `block` (kDmaRows rows) holds.
     const int drow = lane / kRowLanes;
     auto chunk = [&](int block) {
-        return int(swizzled<BK>(kDmaRows * block + drow, lane % kRowLanes));
+        return int(swizzled(kDmaRows * block + drow, lane % kRowLanes));
     };
     const char* xb = reinterpret_cast<const char*>(a.x) + size_t(t0) * a.x_stride;
     const char* wb = reinterpret_cast<const char*>(a.w) + size_t(n0) * a.w_stride;
@@ -248,29 +257,30 @@ w8a8_tiled_kernel(const W8A8Args a) {
         woff[i] = uint32_t(min(kDmaRows * (wave * WI + i) + drow, a.n - 1 - n0)) *
                       uint32_t(a.w_stride) + 16u * chunk(wave * WI + i);
     const uint32_t lds0 = lds_address(s_lds) + ks * L::kPart;
-    const int steps = (a.k + KS * BK - 1) / (KS * BK);
+    const int steps = (a.k + KS * kStep - 1) / (KS * kStep);
     // Workgroups that stream weights of their own begin at different steps: side by side at one
     // k they would ask the same few memory channels for rows a power of two apart, and miss x
     // together (45 x 28672 x 4096: 24.5 to 23.2 us, 32 x 128256 x 4096 89.8 to 87.4). The others
     // share each step's operands in L2 (513 x 4096 x 14336 on 128 x 64 tiles: 83, turned 93).
-    const int turn = a.stream_w ? int(__umulhi(uint32_t(n0 / BN) * 2654435769u, uint32_t(steps))) : 0;
+    const uint32_t spread = uint32_t(n0 / BN) * 2654435769u;  // (2^32 over the golden ratio)
+    const int turn = a.stream_w ? int(__umulhi(spread, uint32_t(steps))) : 0;
     auto issue = [&](int step, int buf) __attribute__((always_inline)) {
         const uint32_t dst = lds0 + buf * L::kStage;
         const int turned = step + turn;
-        const int k0 = ((turned >= steps ? turned - steps : turned) * KS + ks) * BK;
+        const int k0 = ((turned >= steps ? turned - steps : turned) * KS + ks) * kStep;
         const char* xs = xb + k0;
         const char* ws = wb + k0;
-        if (k0 + BK <= a.k) {
+        if (k0 + kStep <= a.k) {
 #pragma unroll
             for (int i = 0; i < XI; ++i) lds_dma16(xs, xoff[i], dst + 1024 * (wave * XI + i));
             if (a.stream_w) {
 #pragma unroll
                 for (int i = 0; i < WI; ++i)
-                    lds_dma16_nt(ws, woff[i], dst + BM * BK + 1024 * (wave * WI + i));
+                    lds_dma16_nt(ws, woff[i], dst + BM * kStep + 1024 * (wave * WI + i));
             } else {
 #pragma unroll
                 for (int i = 0; i < WI; ++i)
-                    lds_dma16(ws, woff[i], dst + BM * BK + 1024 * (wave * WI + i));
+                    lds_dma16(ws, woff[i], dst + BM * kStep + 1024 * (wave * WI + i));
             }
         } else {
             auto in = [&](int block) { return k0 + 16 * chunk(block) < a.k; };
@@ -280,7 +290,8 @@ w8a8_tiled_kernel(const W8A8Args a) {
                 lds_dma16(in(wave * XI + i) ? xs + xoff[i] : zero, dst + 1024 * (wave * XI + i));
 #pragma unroll
             for (int i = 0; i < WI; ++i)
-                lds_dma16(in(wave * WI + i) ? ws + woff[i] : zero, dst + BM * BK + 1024 * (wave * WI + i));
+                lds_dma16(in(wave * WI + i) ? ws + woff[i] : zero,
+                          dst + BM * kStep + 1024 * (wave * WI + i));
         }
     };
 #pragma unroll
@@ -292,7 +303,7 @@ w8a8_tiled_kernel(const W8A8Args a) {
     uint32_t at[Q];
 #pragma unroll
     for (int q = 0; q < Q; ++q)
-        at[q] = uint32_t(col) * BK + 16u * swizzled<BK>(col, C * q + hi);
+        at[q] = uint32_t(col) * kStep + 16u * swizzled(col, C * q + hi);
     typename Mfma<S>::Acc acc[MT][NT];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
@@ -302,14 +313,14 @@ w8a8_tiled_kernel(const W8A8Args a) {
             for (int r = 0; r < 4 * G; ++r) acc[mt][nt][r] = 0;
     int4v_t xf[2][MT], wf[2][NT];
     auto read = [&](int slot, int buf, int q) __attribute__((always_inline)) {
-        const char* sx = s_lds + buf * L::kStage + ks * L::kPart + wm * BK + at[q];
-        const char* sw = sx + (BM + wn - wm) * BK;
+        const char* sx = s_lds + buf * L::kStage + ks * L::kPart + wm * kStep + at[q];
+        const char* sw = sx + (BM + wn - wm) * kStep;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
-            wf[slot][nt] = *reinterpret_cast<const int4v_t*>(sw + nt * S * BK);
+            wf[slot][nt] = *reinterpret_cast<const int4v_t*>(sw + nt * S * kStep);
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
-            xf[slot][mt] = *reinterpret_cast<const int4v_t*>(sx + mt * S * BK);
+            xf[slot][mt] = *reinterpret_cast<const int4v_t*>(sx + mt * S * kStep);
         // (left to itself the compiler moves each read down to its use)
         __builtin_amdgcn_sched_barrier(0);
     };
@@ -332,7 +343,8 @@ w8a8_tiled_kernel(const W8A8Args a) {
             const int e = threadIdx.x + i * THREADS;
             const int t = t0 + e, j = n0 + (e - BM) % BN;
             const float* from = e < BM ? a.xs + t : (e < BM + BN ? a.ws + j : a.bias + j);
-            const bool has = e < BM ? t < a.m : e < BM + 2 * BN && j < a.n && (e < BM + BN || a.bias);
+            const bool has = e < BM ? t < a.m
+                                    : e < BM + 2 * BN && j < a.n && (e < BM + BN || a.bias);
             own[i] = 0.0f;
             if (has) own[i] = *from;
         }
@@ -401,7 +413,8 @@ w8a8_tiled_kernel(const W8A8Args a) {
                 for (int i = 0; i < MT * NT * G; ++i) {
                     const int4v_t v = sums[p * kSlot + i * 64];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[i / G / NT][i / G % NT][4 * (i % G) + e] += v[e];
+                    for (int e = 0; e < 4; ++e)
+                        acc[i / G / NT][i / G % NT][4 * (i % G) + e] += v[e];
                 }
     }
 
@@ -428,7 +441,8 @@ w8a8_tiled_kernel(const W8A8Args a) {
                     if constexpr (sizeof(Y) == 4)
                         *reinterpret_cast<float4*>(to) = make_float4(v0, v1, v2, v3);
                     else
-                        *reinterpret_cast<uint2*>(to) = make_uint2(half_pair(v0, v1), half_pair(v2, v3));
+                        *reinterpret_cast<uint2*>(to) =
+                            make_uint2(half_pair(v0, v1), half_pair(v2, v3));
                 }
         }
         __syncthreads();
@@ -541,7 +555,7 @@ constexpr int kWide = 256;
 
 template <typename Y>
 __global__ __launch_bounds__(512, 2) void w8a8_wide_kernel(const W8A8Args a) {
-    constexpr int BK = 128, WC = 4, kSlot = kWide * BK, kSlots = 5;
+    constexpr int WC = 4, kSlot = kWide * kStep, kSlots = 5;
     constexpr int MT = 4, NT = 2, MF = MT * NT, FR = MT + NT;  // a wave's 32x32 tiles, operands
     constexpr int DI = 4;                                      // a wave's loads of a slot
     __shared__ __align__(16) char s_lds[kSlots * kSlot];
@@ -558,12 +572,12 @@ __global__ __launch_bounds__(512, 2) void w8a8_wide_kernel(const W8A8Args a) {
     int tile = first + (int(blockIdx.x) >> 3);
     if (tile >= end) return;
 
-    const int steps = (a.k + BK - 1) / BK;
-    const int part = a.k % BK / 16;  // chunks of a last, partial step
+    const int steps = (a.k + kStep - 1) / kStep;
+    const int part = a.k % kStep / 16;  // chunks of a last, partial step
     // Instruction i of a slot fetches rows 8 (wave DI + i) .. + 7; the chunk of the lane's place
     // for even and odd i.
     const int drow = lane >> 3;
-    const uint32_t ch0 = swizzled<BK>(drow, lane & 7), ch1 = ch0 ^ 4;
+    const uint32_t ch0 = swizzled(drow, lane & 7), ch1 = ch0 ^ 4;
     const char *xb, *wb;
     uint32_t xoff[DI], woff[DI];
     int t0, n0;
@@ -588,7 +602,7 @@ __global__ __launch_bounds__(512, 2) void w8a8_wide_kernel(const W8A8Args a) {
     const uint32_t back1 = part && ch1 >= uint32_t(part) ? 16 * ch1 : 0;
     auto dma = [&](const char* base, const uint32_t (&off)[DI], int step, int slot, int i)
         __attribute__((always_inline)) {
-        lds_dma16(base + size_t(step) * BK, off[i], lds0 + slot * kSlot + 1024 * i);
+        lds_dma16(base + size_t(step) * kStep, off[i], lds0 + slot * kSlot + 1024 * i);
     };
     auto load = [&](const char* base, const uint32_t (&off)[DI], int step, int slot)
         __attribute__((always_inline)) {
@@ -596,7 +610,7 @@ __global__ __launch_bounds__(512, 2) void w8a8_wide_kernel(const W8A8Args a) {
         const bool cut = part && step + 1 == steps;
 #pragma unroll
         for (int i = 0; i < DI; ++i)
-            lds_dma16(base + size_t(step) * BK, cut ? off[i] - (i & 1 ? back1 : back0) : off[i],
+            lds_dma16(base + size_t(step) * kStep, cut ? off[i] - (i & 1 ? back1 : back0) : off[i],
                       lds0 + slot * kSlot + 1024 * i);
     };
     auto up = [](int slot, int by) { return slot + by >= kSlots ? slot + by - kSlots : slot + by; };
@@ -604,17 +618,17 @@ __global__ __launch_bounds__(512, 2) void w8a8_wide_kernel(const W8A8Args a) {
     const int wm = wave / WC * 128, wn = wave % WC * (kWide / WC);
     uint32_t at[4];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) at[q] = uint32_t(col) * BK + 16u * swizzled<BK>(col, 2 * q + hi);
+    for (int q = 0; q < 4; ++q) at[q] = uint32_t(col) * kStep + 16u * swizzled(col, 2 * q + hi);
     int16v_t acc[MT][NT];
     int4v_t xf[2][MT], wf[2][NT];
     // operand f of sub-step q: the weight rows', then the tokens'
     auto read1 = [&](int p, int xs, int ws, int q, int f) __attribute__((always_inline)) {
         if (f < NT)
-            wf[p][f] = *reinterpret_cast<const int4v_t*>(s_lds + ws * kSlot + wn * BK + at[q] +
-                                                         f * 32 * BK);
+            wf[p][f] = *reinterpret_cast<const int4v_t*>(s_lds + ws * kSlot + wn * kStep + at[q] +
+                                                         f * 32 * kStep);
         else
-            xf[p][f - NT] = *reinterpret_cast<const int4v_t*>(s_lds + xs * kSlot + wm * BK + at[q] +
-                                                              (f - NT) * 32 * BK);
+            xf[p][f - NT] = *reinterpret_cast<const int4v_t*>(
+                s_lds + xs * kSlot + wm * kStep + at[q] + (f - NT) * 32 * kStep);
     };
     auto mfma = [&](int p, int i) __attribute__((always_inline)) {
         acc[i / NT][i % NT] = Mfma<32>::mul(wf[p][i % NT], xf[p][i / NT], acc[i / NT][i % NT]);
@@ -641,7 +655,7 @@ __global__ __launch_bounds__(512, 2) void w8a8_wide_kernel(const W8A8Args a) {
         load(xb, xoff, 2, up(xs, 4));
         fence();
         int st = 0;
-        const int whole = a.k / BK;
+        const int whole = a.k / kStep;
         for (; st + 3 < whole; ++st) {  // the loads that these steps issue are of whole steps
 #pragma unroll
             for (int q = 0; q < 3; ++q)
@@ -705,9 +719,8 @@ __global__ __launch_bounds__(512, 2) void w8a8_wide_kernel(const W8A8Args a) {
             // (waited for here, before the output's stores, which count as later loads do)
             wait_vmcnt<0>();
         }
-        store_wide<Y, MT, NT>(a, c0, c1, lane,
-                              s_lds + (wave < WC ? out : up(out, 1)) * kSlot + wave % WC * (kSlot / WC),
-                              acc);
+        char* mine = s_lds + (wave < WC ? out : up(out, 1)) * kSlot + wave % WC * (kSlot / WC);
+        store_wide<Y, MT, NT>(a, c0, c1, lane, mine, acc);
         if (!more) return;
         xs = up(xs, 2);
     }
@@ -715,26 +728,27 @@ __global__ __launch_bounds__(512, 2) void w8a8_wide_kernel(const W8A8Args a) {
 
 template <typename Y, int R, int U>
 void launch_row(const W8A8Args& a, hipStream_t s) {
-    hipLaunchKernelGGL((w8a8_row_kernel<Y, R, U>), dim3((a.n + kRowWaves * R - 1) / (kRowWaves * R)),
-                       dim3(64 * kRowWaves), 0, s, a);
+    const int per = kRowWaves * R;
+    hipLaunchKernelGGL((w8a8_row_kernel<Y, R, U>), dim3((a.n + per - 1) / per), dim3(64 * kRowWaves),
+                       0, s, a);
 }
 
-template <typename Y, int S, int BM, int BN, int WR, int WC, int KS, int BK, int ST, int WGS>
+template <typename Y, int S, int BM, int BN, int WR, int WC, int KS, int ST, int WGS>
 void launch_tiled(const W8A8Args& a, hipStream_t s) {
     const int mb = (a.m + BM - 1) / BM, tiles = mb * ((a.n + BN - 1) / BN);
     W8A8Args b = a;
     // Weights that one row of tiles reads are streamed, as the FP8 GEMV streams its own: those
     // under 12 MB may stay in the caches from one launch to the next.
     b.stream_w = mb == 1 && int64_t(a.n) * a.k > 12 << 20;
-    hipLaunchKernelGGL((w8a8_tiled_kernel<Y, S, BM, BN, WR, WC, KS, BK, ST, WGS>), dim3(tiles),
+    hipLaunchKernelGGL((w8a8_tiled_kernel<Y, S, BM, BN, WR, WC, KS, ST, WGS>), dim3(tiles),
                        dim3(64 * WR * WC * KS), 0, s, b);
 }
 
 template <typename Y>
 void launch_wide(const W8A8Args& a, hipStream_t s) {
     const int tiles = ((a.m + kWide - 1) / kWide) * ((a.n + kWide - 1) / kWide);
-    hipLaunchKernelGGL(w8a8_wide_kernel<Y>, dim3(std::min(tiles, device_compute_units())), dim3(512),
-                       0, s, a);
+    const int wgs = std::min(tiles, device_compute_units());
+    hipLaunchKernelGGL(w8a8_wide_kernel<Y>, dim3(wgs), dim3(512), 0, s, a);
 }
 
 // The forms (token rows, weight rows, parts of K, workgroups per CU), and what a launch of
@@ -775,7 +789,7 @@ int pick_form(const W8A8Args& a) {
     // (called for every launch: constant tile sizes, 32-bit arithmetic; tiles are below 2^29)
     const unsigned cus = unsigned(device_compute_units());
     const unsigned m = unsigned(a.m), n = unsigned(a.n), k = unsigned(a.k);
-    const float mb = float(a.n) * float(a.k) * 1e-6f;
+    const float weights = float(a.n) * float(a.k) * 1e-6f;  // MB
     int best = 0;
     float best_cost = 0.0f;
 #pragma clang loop unroll(full)
@@ -785,9 +799,9 @@ int pick_form(const W8A8Args& a) {
         const unsigned tiles = up(m, c.bm) * up(n, c.bn);
         const unsigned per_cu = (tiles + cus - 1) / cus;  // of the busiest CUs
         const float steps = float(up(k, 128 * c.ks));
+        const float all = float(tiles) / float(cus);
         const float cost = c.fixed + float(up(per_cu, c.wgs)) * (c.round + steps * c.step) +
-                           steps * (float(per_cu) * c.share + float(tiles) / float(cus) * c.spread) +
-                           mb * c.stream;
+                           steps * (float(per_cu) * c.share + all * c.spread) + weights * c.stream;
         if (i == 0 || cost < best_cost) {
             best = i;
             best_cost = cost;
@@ -803,20 +817,20 @@ void launch_w8a8(const W8A8Args& a, hipStream_t s) {
     // 11.2 / 10.8; the best tiles 6.7, 20.9 and 11.5.)
     if (a.m == 1) return a.k <= 4096 ? launch_row<Y, 1, 4>(a, s) : launch_row<Y, 2, 4>(a, s);
     switch (pick_form(a)) {
-        case k16x16k8: return launch_tiled<Y, 16, 16, 16, 1, 1, 8, 128, 4, 1>(a, s);
-        case k16x32k4: return launch_tiled<Y, 16, 16, 32, 1, 1, 4, 128, 3, 2>(a, s);
-        case k32x32k4: return launch_tiled<Y, 32, 32, 32, 1, 1, 4, 128, 4, 1>(a, s);
-        case k32x64k2: return launch_tiled<Y, 32, 32, 64, 1, 2, 2, 128, 3, 2>(a, s);
-        case k64x32k4: return launch_tiled<Y, 32, 64, 32, 2, 1, 4, 128, 3, 1>(a, s);
-        case k64x64k2: return launch_tiled<Y, 32, 64, 64, 2, 2, 2, 128, 4, 1>(a, s);
-        case k128x64k2: return launch_tiled<Y, 32, 128, 64, 2, 2, 2, 128, 3, 1>(a, s);
-        case k128x96: return launch_tiled<Y, 32, 128, 96, 4, 1, 1, 128, 4, 1>(a, s);
-        case k128x128: return launch_tiled<Y, 32, 128, 128, 4, 2, 1, 128, 3, 1>(a, s);
-        case k192x128: return launch_tiled<Y, 32, 192, 128, 2, 4, 1, 128, 3, 1>(a, s);
+        case k16x16k8: return launch_tiled<Y, 16, 16, 16, 1, 1, 8, 4, 1>(a, s);
+        case k16x32k4: return launch_tiled<Y, 16, 16, 32, 1, 1, 4, 3, 2>(a, s);
+        case k32x32k4: return launch_tiled<Y, 32, 32, 32, 1, 1, 4, 4, 1>(a, s);
+        case k32x64k2: return launch_tiled<Y, 32, 32, 64, 1, 2, 2, 3, 2>(a, s);
+        case k64x32k4: return launch_tiled<Y, 32, 64, 32, 2, 1, 4, 3, 1>(a, s);
+        case k64x64k2: return launch_tiled<Y, 32, 64, 64, 2, 2, 2, 4, 1>(a, s);
+        case k128x64k2: return launch_tiled<Y, 32, 128, 64, 2, 2, 2, 3, 1>(a, s);
+        case k128x96: return launch_tiled<Y, 32, 128, 96, 4, 1, 1, 4, 1>(a, s);
+        case k128x128: return launch_tiled<Y, 32, 128, 128, 4, 2, 1, 3, 1>(a, s);
+        case k192x128: return launch_tiled<Y, 32, 192, 128, 2, 4, 1, 3, 1>(a, s);
         case k256x256: return launch_wide<Y>(a, s);
-        case k192x256: return launch_tiled<Y, 32, 192, 256, 2, 4, 1, 128, 2, 1>(a, s);
-        case k64x128: return launch_tiled<Y, 32, 64, 128, 2, 2, 1, 128, 3, 2>(a, s);
-        case k128x128x2: return launch_tiled<Y, 32, 128, 128, 2, 2, 1, 128, 2, 2>(a, s);
+        case k192x256: return launch_tiled<Y, 32, 192, 256, 2, 4, 1, 2, 1>(a, s);
+        case k64x128: return launch_tiled<Y, 32, 64, 128, 2, 2, 1, 3, 2>(a, s);
+        case k128x128x2: return launch_tiled<Y, 32, 128, 128, 2, 2, 1, 2, 2>(a, s);
     }
 }
 

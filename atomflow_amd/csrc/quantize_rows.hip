@@ -96,7 +96,8 @@ __device__ __forceinline__ void store8(float* p, int e, int n, const float (&v)[
 // number, to nearest even (the sum's last place is 1), and leaves that in the low byte. The
 // product is rounded by itself, as written in the formula, so that a program that computes it
 // in fp32 gets the same codes.
-__device__ __forceinline__ void store_codes(int8_t* p, int e, int n, const float (&v)[8], float inv) {
+__device__ __forceinline__ void store_codes(int8_t* p, int e, int n, const float (&v)[8],
+                                            float inv) {
 #pragma clang fp contract(off)
     uint32_t b[8];
 #pragma unroll
@@ -340,7 +341,8 @@ void launch_slice(const RowArgs& a, hipStream_t s) {
     else if (a.n <= 1024) launch_rows<MODE, 64, 2>(a, s);
     else if (a.n <= 2048) launch_rows<MODE, 256, 1>(a, s);
     else if (a.n <= 4096) launch_rows<MODE, 512, 1>(a, s);
-    else if (a.n <= 8192 && (few || (MODE != kPlain && a.n > 7168))) launch_rows<MODE, 1024, 1>(a, s);
+    else if (a.n <= 8192 && (few || (MODE != kPlain && a.n > 7168)))
+        launch_rows<MODE, 1024, 1>(a, s);
     else if (a.n <= 8192) launch_rows<MODE, 512, 2>(a, s);
     else if (a.n <= 16384) launch_rows<MODE, 1024, 2>(a, s);
     else if (a.n <= 32768) launch_rows<MODE, 1024, 4>(a, s);
