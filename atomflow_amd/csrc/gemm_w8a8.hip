@@ -752,37 +752,40 @@ void launch_wide(const W8A8Args& a, hipStream_t s) {
 }
 
 // The forms (token rows, weight rows, parts of K, workgroups per CU), and what a launch of
-// each was measured to cost on MI355X (eleven (n, k) shapes from 1024 x 1024 to 128256 x 4096, 2
+// each was measured to cost on MI355X (21 (n, k) shapes from 8192 x 64 to 151936 x 2048, 2
 // to 4096 tokens, weights read from HBM): a round of workgroups, `wgs` of them per CU while
 // tiles last, takes `round` plus per step (128 k of each part) `step`, for each workgroup of
 // the busiest CUs `share` and of the average CU `spread` (us); a launch `fixed` besides, and
 // `stream` per MB of weights. Small tiles with several parts of K at a time fill the device
 // when tokens or rows are few, large ones read the least and keep the matrix cores busiest.
-// The rule picks a form within 1 % of the best measured one on average (16 % at most).
+// The rule picks a form within 1.5 % of the best measured one on average (23 % at most).
 struct TileCost {
     int bm, bn, ks, wgs;
     float fixed, round, step, share, spread, stream;
 };
 enum {
-    k16x16k8, k16x32k4, k32x32k4, k32x64k2, k64x32k4, k64x64k2, k128x64k2,
-    k128x96, k128x128, k192x128, k256x256, k192x256, k64x128, k128x128x2,
+    k16x16k8, k16x32k4, k32x32k4, k32x64k2, k64x32k4, k64x64x2, k64x64k2,
+    k128x64k2, k128x96, k128x128, k192x128, k256x256, k192x256, k64x128,
+    k128x128x2, k32x256,
     kForms
 };
 constexpr TileCost kTileCost[kForms] = {
-    {16, 16, 8, 1, 1.7120f, 1.1334f, 0.2359f, 0.0f, 0.2412f, 0.0435f},
-    {16, 32, 4, 2, 2.1473f, 0.7189f, 0.0231f, 0.2282f, 0.0638f, 0.0730f},
-    {32, 32, 4, 1, 1.7303f, 1.5279f, 0.3059f, 0.0f, 0.1797f, 0.0421f},
-    {32, 64, 2, 2, 1.9726f, 0.9416f, 0.1054f, 0.2219f, 0.0798f, 0.0592f},
-    {64, 32, 4, 1, 1.3493f, 2.0178f, 0.5190f, 0.0f, 0.0958f, 0.0739f},
-    {64, 64, 2, 1, 1.3464f, 2.1042f, 0.4067f, 0.0f, 0.0729f, 0.0572f},
-    {128, 64, 2, 1, 1.8117f, 2.6802f, 0.5523f, 0.0f, 0.1929f, 0.0425f},
-    {128, 96, 1, 1, 1.7855f, 3.5270f, 0.3845f, 0.0f, 0.0958f, 0.0345f},
-    {128, 128, 1, 1, 1.4190f, 2.9689f, 0.4229f, 0.0f, 0.1518f, 0.0494f},
-    {192, 128, 1, 1, 1.6542f, 4.3061f, 0.4765f, 0.0f, 0.2935f, 0.0317f},
-    {256, 256, 1, 1, 0.8484f, 7.4613f, 0.9766f, 0.0f, 0.5346f, 0.0563f},
-    {192, 256, 1, 1, 2.1602f, 5.8443f, 0.8915f, 0.0f, 0.4288f, 0.0438f},
-    {64, 128, 1, 2, 2.5805f, 1.7073f, 0.1050f, 0.1910f, 0.1032f, 0.0660f},
-    {128, 128, 1, 2, 0.9998f, 3.9925f, 0.5376f, 0.0343f, 0.2072f, 0.0570f}
+    {16, 16, 8, 1, 1.5253f, 1.1634f, 0.2820f, 0.0f, 0.2026f, 0.0435f},
+    {16, 32, 4, 2, 1.6584f, 1.0537f, 0.0427f, 0.2422f, 0.0421f, 0.0677f},
+    {32, 32, 4, 1, 1.4628f, 1.5650f, 0.3373f, 0.0f, 0.1539f, 0.0428f},
+    {32, 64, 2, 2, 1.5800f, 1.3526f, 0.1062f, 0.2143f, 0.0824f, 0.0599f},
+    {64, 32, 4, 1, 1.1681f, 2.0336f, 0.5269f, 0.0f, 0.1022f, 0.0762f},
+    {64, 64, 1, 2, 1.1423f, 2.1340f, 0.0735f, 0.1634f, 0.0245f, 0.0575f},
+    {64, 64, 2, 1, 1.1364f, 2.1727f, 0.4097f, 0.0f, 0.0791f, 0.0573f},
+    {128, 64, 2, 1, 1.5647f, 2.7491f, 0.5400f, 0.0f, 0.2365f, 0.0436f},
+    {128, 96, 1, 1, 1.4953f, 3.6545f, 0.3755f, 0.0f, 0.1381f, 0.0299f},
+    {128, 128, 1, 1, 1.0881f, 3.0483f, 0.4148f, 0.0f, 0.1950f, 0.0440f},
+    {192, 128, 1, 1, 1.5970f, 3.7784f, 0.4931f, 0.0f, 0.3379f, 0.0246f},
+    {256, 256, 1, 1, 1.2085f, 6.8190f, 0.9115f, 0.0f, 0.6966f, 0.0614f},
+    {192, 256, 1, 1, 2.0918f, 5.7229f, 0.8791f, 0.0f, 0.5041f, 0.0339f},
+    {64, 128, 1, 2, 1.4440f, 2.5838f, 0.0989f, 0.2060f, 0.0959f, 0.0652f},
+    {128, 128, 1, 2, 0.8969f, 4.2947f, 0.4938f, 0.0303f, 0.2533f, 0.0530f},
+    {32, 256, 1, 2, 1.3309f, 2.1394f, 0.4646f, 0.1685f, 0.1281f, 0.0776f}
 };
 
 int pick_form(const W8A8Args& a) {
@@ -822,6 +825,7 @@ void launch_w8a8(const W8A8Args& a, hipStream_t s) {
         case k32x32k4: return launch_tiled<Y, 32, 32, 32, 1, 1, 4, 4, 1>(a, s);
         case k32x64k2: return launch_tiled<Y, 32, 32, 64, 1, 2, 2, 3, 2>(a, s);
         case k64x32k4: return launch_tiled<Y, 32, 64, 32, 2, 1, 4, 3, 1>(a, s);
+        case k64x64x2: return launch_tiled<Y, 32, 64, 64, 2, 2, 1, 4, 2>(a, s);
         case k64x64k2: return launch_tiled<Y, 32, 64, 64, 2, 2, 2, 4, 1>(a, s);
         case k128x64k2: return launch_tiled<Y, 32, 128, 64, 2, 2, 2, 3, 1>(a, s);
         case k128x96: return launch_tiled<Y, 32, 128, 96, 4, 1, 1, 4, 1>(a, s);
@@ -831,6 +835,7 @@ void launch_w8a8(const W8A8Args& a, hipStream_t s) {
         case k192x256: return launch_tiled<Y, 32, 192, 256, 2, 4, 1, 2, 1>(a, s);
         case k64x128: return launch_tiled<Y, 32, 64, 128, 2, 2, 1, 3, 2>(a, s);
         case k128x128x2: return launch_tiled<Y, 32, 128, 128, 2, 2, 1, 2, 2>(a, s);
+        case k32x256: return launch_tiled<Y, 32, 32, 256, 1, 4, 1, 2, 2>(a, s);
     }
 }
 

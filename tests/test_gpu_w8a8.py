@@ -305,7 +305,12 @@ FORMS = [(1, 4100, 14352), (1, 33, 4112), (1, 37, 131056), (2, 54, 14352), (33, 
          (4679, 385, 208), (196, 8792, 48), (539, 10659, 528), (266, 13342, 1552),
          (515, 14499, 48), (525, 14634, 144), (586, 13115, 400), (513, 14851, 528),
          (67, 10881, 16), (69, 11088, 400), (4131, 201, 1552), (65, 11432, 1040),
-         (259, 13824, 16), (325, 10899, 48), (261, 13611, 400), (385, 11597, 1040)]
+         (259, 13824, 16), (325, 10899, 48), (261, 13611, 400), (385, 11597, 1040),
+         (34, 8295, 1024), (33, 8532, 14352), (33, 11148, 400), (71, 11082, 2080),
+         (65, 10997, 4096), (135, 11087, 14352), (1283, 12683, 16), (259, 14429, 144),
+         (322, 11060, 528), (642, 12292, 16), (513, 13126, 1024), (129, 8507, 14352),
+         (4129, 788, 16), (265, 14548, 16), (404, 11022, 400), (2725, 1411, 208),
+         (385, 9362, 528), (31, 125003, 1040)]
 WIDE = [(986, 11095, 16), (991, 10899, 48), (981, 10949, 128), (812, 13272, 144), (965, 11011, 256),
         (965, 10859, 384), (806, 13146, 400), (777, 13348, 528), (1001, 10996, 1552),
         (3670, 6695, 16), (1818, 13482, 48), (3588, 6882, 128), (2182, 11239, 144),
