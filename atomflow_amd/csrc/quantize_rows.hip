@@ -92,17 +92,24 @@ __device__ __forceinline__ void store8(float* p, int e, int n, const float (&v)[
     }
 }
 
-// Codes of v: v * inv is within 2^-23 of v * 127 / a; adding 1.5 * 2^23 rounds it to a whole
-// number, to nearest even (the sum's last place is 1), and leaves that in the low byte. The
-// product is rounded by itself, as written in the formula, so that a program that computes it
-// in fp32 gets the same codes.
+// Codes of v: adding 1.5 * 2^23 to a quotient rounds it to a whole number, to nearest even (the
+// sum's last place is 1), and leaves that in the low byte.
+//
+// Computed values (v is rounded itself): the quotient is v * inv, within 2^-23 of v * 127 / a,
+// rounded by itself, so that a program that computes the formula in fp32 gets the same codes.
+// Plain rows (EXACT): v and a are fp16, and quotients that lie halfway between two codes are
+// common (v = a / 2 is 63.5), so the rounding of inv would choose between them. With the rest
+// of 127 / a in inv_lo the quotient is the exact one to nearest: a half stays a half, and what
+// is none is at least 16 times that rounding away from one (v has 11 bits, a too). It costs
+// 1 to 3 % (8192 rows of 8192 36.5 -> 37.2 us).
+template <bool EXACT>
 __device__ __forceinline__ void store_codes(int8_t* p, int e, int n, const float (&v)[8],
-                                            float inv) {
+                                            float inv, float inv_lo) {
 #pragma clang fp contract(off)
     uint32_t b[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const float q = v[i] * inv;
+        const float q = EXACT ? __builtin_fmaf(v[i], inv, v[i] * inv_lo) : v[i] * inv;
         b[i] = __builtin_bit_cast(uint32_t, q + 12582912.0f);
     }
     if (e + 8 <= n) {
@@ -198,6 +205,7 @@ __device__ __forceinline__ float norm_factor(float sum, const RowArgs& a) {
 struct Scale {
     float inv, scale;
     bool bad;
+    float inv_lo;  // of 127 / a, what inv's rounding leaves
 };
 __device__ __forceinline__ Scale row_scale(uint32_t bits) {
     const float top = __builtin_bit_cast(float, bits);
@@ -205,6 +213,7 @@ __device__ __forceinline__ Scale row_scale(uint32_t bits) {
     Scale r;
     r.bad = bits >= 0x7f800000u;
     r.inv = zero ? 0.0f : 127.0f / top;
+    r.inv_lo = zero ? 0.0f : __builtin_fmaf(-r.inv, top, 127.0f) / top;
     r.scale = r.bad ? __builtin_nanf("") : (zero ? 1.0f : top / 127.0f);
     return r;
 }
@@ -258,8 +267,8 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void rows_kernel(const RowArgs a
         if (sc.bad)
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[c][i] = 0.0f;
-        store_codes(a.codes + row * a.codes_stride, 8 * (t + c * T), a.n, v[c],
-                    sc.bad ? 0.0f : sc.inv);
+        store_codes<MODE == kPlain>(a.codes + row * a.codes_stride, 8 * (t + c * T), a.n, v[c],
+                                    sc.bad ? 0.0f : sc.inv, sc.bad ? 0.0f : sc.inv_lo);
     }
     if (t == 0) a.scales[row] = sc.scale;
 }
@@ -293,7 +302,7 @@ __global__ __launch_bounds__(1024) void long_rows_kernel(const RowArgs a) {
             for (int i = 0; i < 8; ++i) v[i] = v[i] * f * w[i];
         }
     };
-    Scale sc{0.0f, 1.0f, false};
+    Scale sc{0.0f, 1.0f, false, 0.0f};
     if (a.codes) {
         uint32_t top = 0;
         for (int e = 8 * threadIdx.x; e < a.n; e += 8 * 1024) {
@@ -313,7 +322,8 @@ __global__ __launch_bounds__(1024) void long_rows_kernel(const RowArgs a) {
             if (sc.bad)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-            store_codes(a.codes + row * a.codes_stride, e, a.n, v, sc.bad ? 0.0f : sc.inv);
+            store_codes<MODE == kPlain>(a.codes + row * a.codes_stride, e, a.n, v,
+                                        sc.bad ? 0.0f : sc.inv, sc.bad ? 0.0f : sc.inv_lo);
         }
     }
 }
@@ -332,7 +342,7 @@ void launch_rows(const RowArgs& a, hipStream_t s) {
 // rows take a wave each, which needs no barrier: 8192 rows of 1024 8.2 / 13.1 / 15.1, on 256
 // threads 9.9 / 13.5 / 17.5. Above 4096, 1024 threads suit few rows (45 of 5120: 2.4 / 3.0 /
 // 3.7, on 512 threads 2.6 / 3.5 / 4.2), and many only where the row fills them (8192 of 8192:
-// 40.9 / 61.7 / 85.0 and 36.8 / 62.1 / 88.1; of 5120: 34.0 / 47.8 / 66.1 and 26.8 / 43.4 / 59.4).
+// 40.9 / 61.7 / 85.0 and 37.2 / 62.1 / 88.1; of 5120: 34.0 / 47.8 / 66.1 and 26.8 / 43.4 / 59.4).
 // 85.0 us are 5.5 TB/s, what a large copy reaches on this card (5.15) and more.
 template <int MODE>
 void launch_slice(const RowArgs& a, hipStream_t s) {

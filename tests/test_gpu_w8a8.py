@@ -103,6 +103,33 @@ def test_quantize_rows(gpu, n, m, off):
     assert np.array_equal(scales[good], want[good])
 
 
+def exact_codes(x):
+    """Codes of fp16 rows in whole numbers: 127 * v / a to nearest, halves to even."""
+    v = np.rint(x.astype(np.float64) * 2.0 ** 24).astype(np.int64)  # (fp16 is a multiple of 2^-24)
+    a = np.abs(v).max(axis=1, keepdims=True)
+    num, den = 254 * np.abs(v), 2 * np.maximum(a, 1)
+    q, rest = num // den, 2 * (num % den)
+    return np.sign(v) * (q + ((rest > den) | ((rest == den) & (q % 2 == 1))))
+
+
+@pytest.mark.parametrize("m,n", [(600, 512), (40, 1024), (300, 4096), (9, 8192), (5, 40000)])
+def test_quantize_rows_halves(gpu, m, n):
+    """Quotients halfway between two codes are common in fp16 rows: halves, and other odd
+    multiples of a / 254, of the row's largest value. Codes are those of exact arithmetic."""
+    say(f"quantize rows, halves m={m} n={n}")
+    r = np.random.default_rng(m + n)
+    top = np.exp2(r.uniform(-22, 15.9, (m, 1))).astype(np.float16)
+    odd = 2 * r.integers(-127, 127, (m, n)) + 1
+    x = (odd * (top.astype(np.float64) / 254)).astype(np.float16)
+    x[:, 1::5] = (r.uniform(-1, 1, x[:, 1::5].shape) * top).astype(np.float16)
+    x[:, 2::7] = np.where(odd[:, 2::7] > 0, top / np.float16(2), top / np.float16(-2))
+    x[:, :1] = top
+    xr = Rows(np.float16, m, n, n, 0, x)
+    c, s = Rows(np.int8, m, n, n), Rows(np.float32, m, 1, 1)
+    kv.launch_quantize_rows(xr.ptr, xr.stride, m, n, c.ptr, c.stride, s.ptr)
+    assert np.array_equal(c.get(), exact_codes(x))
+
+
 @pytest.mark.parametrize("n", WIDTHS)
 @pytest.mark.parametrize("m,off,fused", [(1, 0, True), (9, 1, False), (33, 0, True)])
 def test_silu_mul_quantize(gpu, n, m, off, fused):
