@@ -134,9 +134,10 @@ __global__ __launch_bounds__(64 * kRowWaves) void w8a8_row_kernel(const W8A8Args
 //
 // What bounds it, between a few dozen and a few hundred tokens, is the loads: 8 rows of 128
 // bytes an instruction reach 98 GB/s per CU from L2 (1 KB pieces 145), and HBM's latency. 513
-// x 4096 x 14336 runs in 60 us with the matrix cores busy a quarter of the time; stages twice
-// as many or as long, operands a whole step ahead, and a wave that touches the weights' lines
-// early gave nothing or cost time.
+// x 4096 x 14336 runs in 60 us (weights from HBM) with the matrix cores busy a quarter of the
+// time; stages twice as many or as long, operands a whole step ahead, waves of 64 x 64 and 64 x
+// 96 (which read a third less from LDS), and a wave that touches the weights' lines early gave
+// nothing or cost time.
 constexpr int kStep = 128;
 
 // lds_dma16 of a wave-uniform base and lane offsets, non-temporal.
@@ -260,8 +261,10 @@ w8a8_tiled_kernel(const W8A8Args a) {
     const int steps = (a.k + KS * kStep - 1) / (KS * kStep);
     // Workgroups that stream weights of their own begin at different steps: side by side at one
     // k they would ask the same few memory channels for rows a power of two apart, and miss x
-    // together (45 x 28672 x 4096: 24.5 to 23.2 us, 32 x 128256 x 4096 89.8 to 87.4). The others
-    // share each step's operands in L2 (513 x 4096 x 14336 on 128 x 64 tiles: 83, turned 93).
+    // together (45 x 28672 x 4096: 27.9 to 21.6 us, 32 x 128256 x 4096 118 to 79; without the
+    // non-temporal loads too, 31 and 127). The others share each step's operands in L2: turned,
+    // launches of two to four token tiles took 9 % less to 24 % more time, of five and more up
+    // to a third more (513 x 4096 x 14336 on 128 x 64 tiles: 82 and 92).
     const uint32_t spread = uint32_t(n0 / BN) * 2654435769u;  // (2^32 over the golden ratio)
     const int turn = a.stream_w ? int(__umulhi(spread, uint32_t(steps))) : 0;
     auto issue = [&](int step, int buf) __attribute__((always_inline)) {

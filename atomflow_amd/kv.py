@@ -95,8 +95,7 @@ def launch_qkv_rope_append(x, w_qkv, scales, k, qkv_out, k_cache, v_cache, cos_t
                                    _p(d_status), _s(stream)), "launch_qkv_rope_append")
 
 
-# ---- prefill (multi-token append, causal attention over a prompt chunk) -----
-# ---- 8-bit integer projections -------------------------------------------------
+# ---- 8-bit integer projections -----------------------------------------------
 def launch_quantize_rows(x, x_stride, m, n, codes, codes_stride, scales, stream=None):
     """fp16 rows to int8 codes with one fp32 scale per row (scale = max |x| / 127)."""
     check(lib().af_quantize_rows(_p(x), x_stride, m, n, _p(codes), codes_stride, _p(scales),
@@ -129,6 +128,7 @@ def launch_w8a8_gemm(x, x_stride, x_scales, m, weight, w_stride, w_scales, y, y_
           "launch_w8a8_gemm")
 
 
+# ---- prefill (multi-token append, causal attention over a prompt chunk) -----
 def launch_prefill_rope_append(qkv_out, n, k_cache, v_cache, cos_table, sin_table, p0, max_seq,
                                n_q_heads, n_kv_heads, head_dim, d_p0=None, d_status=None,
                                stream=None):

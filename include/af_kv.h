@@ -407,8 +407,9 @@ int af_silu_mul_quantize(const void* gate, const void* up, int64_t stride, int m
  * NULL, not both. The norm is of the unrounded fp32 sum s. residual NULL (and
  * residual_out NULL): v is the norm of x. residual_dtype: AF_FP16 or AF_FP32
  * (both residual pointers; rows residual_stride elements apart). residual_out
- * may be residual itself. weight: fp32 [n]; 0 < eps < infinity. A row whose sum of squares is not finite in fp32
- * counts as one that holds a NaN (normed is NaN; residual_out is s). */
+ * may be residual itself. weight: fp32 [n]; 0 < eps < infinity. A row whose sum of
+ * squares is not finite in fp32 counts as one that holds a NaN (normed is NaN;
+ * residual_out is s). */
 int af_rmsnorm_quantize(const void* x, int64_t x_stride, const void* residual, void* residual_out,
                         int64_t residual_stride, int residual_dtype, const float* weight, float eps,
                         int m, int n, int8_t* codes, int64_t codes_stride, float* scales,
