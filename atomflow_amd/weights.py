@@ -82,8 +82,12 @@ def quantize_int8(w):
         raise ValueError("weights hold values that are not finite")
     top = np.abs(t).max(axis=1, initial=0.0).astype(np.float64)
     zero = top < 2.0 ** -100
+    q = t.astype(np.float64)
+    q *= 127.0  # exact, and the quotient rounds once: halves of a step stay halves
+    q /= np.where(zero, 1.0, top)[:, None]
+    q[zero] = 0.0
     codes = np.zeros((t.shape[0], -(-t.shape[1] // 16) * 16), np.int8)
-    codes[:, :t.shape[1]] = np.rint(np.where(zero, 0.0, 127.0 / np.where(zero, 1.0, top))[:, None] * t)
+    codes[:, :t.shape[1]] = np.rint(q, out=q)
     return codes, np.where(zero, 1.0, top / 127.0).astype(np.float32)
 
 

@@ -382,7 +382,8 @@ int af_qkv_rope_append(const void* x, const uint8_t* w_qkv, const void* scales, 
 
 /* Rows of int8 codes with one fp32 scale each: element value = code * scale.
  * For a row v: a = max |v|, scale = a / 127, code = v * 127 / a rounded to
- * nearest even, so codes are within +-127. A row of zeros (or of magnitudes
+ * nearest even (the exact quotient where v is x itself, the fp32 product
+ * v * (127 / a) where v is computed), so codes are within +-127. A row of zeros (or of magnitudes
  * below 2^-100) gets codes 0 and scale 1. A row that holds a NaN or an infinity
  * gets codes 0 and scale NaN: what is computed from it is NaN.
  * codes: row i at codes + i * codes_stride (bytes past n of a row are left as

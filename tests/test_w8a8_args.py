@@ -167,6 +167,20 @@ def test_quantize_int8(n, k):
     w8a8_ref.assert_codes(codes[:, :k], scales, w.astype(np.float64), 0.0)
 
 
+def test_quantize_int8_halves():
+    """Odd multiples of a / 254 lie halfway between two codes: to the even one, whatever a is."""
+    r = np.random.default_rng(5)
+    unit = r.integers(1, 1 << 15, (300, 1)) * np.exp2(r.integers(-40, 20, (300, 1)))
+    odd = 2 * r.integers(-127, 127, (300, 64)) + 1
+    w = (odd * unit).astype(np.float32)  # exact
+    w[:, 7] = 254 * unit[:, 0]
+    codes, scales = weights.quantize_int8(w)
+    want = np.rint(odd / 2.0)
+    want[:, 7] = 127
+    assert np.array_equal(codes, want)
+    assert np.array_equal(scales, (2 * unit[:, 0]).astype(np.float32))
+
+
 def test_quantize_int8_refuses():
     for bad in (np.zeros(4), np.full((2, 3), np.nan), np.array([[1.0, np.inf]])):
         with pytest.raises(ValueError):
