@@ -149,17 +149,21 @@ __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
     return a > b ? a : b;
 }
 
-// One value per wave of the row to all of the row's threads, combined in wave order.
-template <int WAVES, typename V, typename F>
-__device__ __forceinline__ V across_waves(V v, V* s, F op) {
+// One value per wave of the row (or one for each of P chunks) to all of the row's threads,
+// combined in the order of chunks and waves.
+template <int WAVES, int P, typename V, typename F>
+__device__ __forceinline__ V across_waves(const V (&v)[P], V* s, F op) {
     if constexpr (WAVES == 1) {
-        return v;
+        static_assert(P == 1, "one value");
+        return v[0];
     } else {
-        if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
+        if ((threadIdx.x & 63) == 0)
+#pragma unroll
+            for (int p = 0; p < P; ++p) s[p * WAVES + (threadIdx.x >> 6)] = v[p];
         __syncthreads();
         V r = s[0];
 #pragma unroll
-        for (int i = 1; i < WAVES; ++i) r = op(r, s[i]);
+        for (int i = 1; i < P * WAVES; ++i) r = op(r, s[i]);
         return r;
     }
 }
@@ -223,7 +227,10 @@ __device__ __forceinline__ Scale row_scale(uint32_t bits) {
 template <int MODE, int T, int CH>
 __global__ __launch_bounds__(T < 256 ? 256 : T) void rows_kernel(const RowArgs a) {
     constexpr int WAVES = T / 64, ROWS = T < 256 ? 256 / T : 1;
-    __shared__ float s_sum[WAVES];
+    // Rows that few of them give 1024 threads and many 512 with two chunks each are summed in
+    // the first's order by both, so that a row's bits do not depend on how many there are.
+    constexpr int SUMS = T == 512 ? CH : 1;
+    __shared__ float s_sum[SUMS * WAVES];
     __shared__ uint32_t s_max[WAVES];
     const int t = threadIdx.x % T;
     const int row_i = int(blockIdx.x) * ROWS + int(threadIdx.x) / T;
@@ -233,19 +240,22 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void rows_kernel(const RowArgs a
 #pragma unroll
     for (int c = 0; c < CH; ++c) load_chunk<MODE>(a, row, 8 * (t + c * T), v[c]);
     if constexpr (MODE >= kNorm) {
-        float sum = 0.0f;
+        float sums[SUMS] = {};
 #pragma unroll
         for (int c = 0; c < CH; ++c)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum = fmaf(v[c][i], v[c][i], sum);
+            for (int i = 0; i < 8; ++i)
+                sums[c % SUMS] = fmaf(v[c][i], v[c][i], sums[c % SUMS]);
         float w[CH][8];
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             load8(a.weight, 8 * (t + c * T), a.n, w[c]);
             store_residual<MODE>(a, row, 8 * (t + c * T), v[c]);
         }
-        sum = across_waves<WAVES>(wave_sum(sum), s_sum, [](float p, float q) { return p + q; });
-        const float f = norm_factor(sum, a);
+#pragma unroll
+        for (int i = 0; i < SUMS; ++i) sums[i] = wave_sum(sums[i]);
+        const float f = norm_factor(
+            across_waves<WAVES>(sums, s_sum, [](float p, float q) { return p + q; }), a);
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
 #pragma unroll
@@ -254,14 +264,14 @@ __global__ __launch_bounds__(T < 256 ? 256 : T) void rows_kernel(const RowArgs a
         }
         if (!a.codes) return;
     }
-    uint32_t top = 0;
+    uint32_t top[1] = {0};
 #pragma unroll
     for (int c = 0; c < CH; ++c)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) top = max(top, magnitude(v[c][i]));
-    top = across_waves<WAVES>(wave_max_u32(top), s_max,
-                              [](uint32_t p, uint32_t q) { return p > q ? p : q; });
-    const Scale sc = row_scale(top);
+        for (int i = 0; i < 8; ++i) top[0] = max(top[0], magnitude(v[c][i]));
+    top[0] = wave_max_u32(top[0]);
+    const Scale sc = row_scale(across_waves<WAVES>(
+        top, s_max, [](uint32_t p, uint32_t q) { return p > q ? p : q; }));
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
         if (sc.bad)
@@ -284,14 +294,14 @@ __global__ __launch_bounds__(1024) void long_rows_kernel(const RowArgs a) {
     float f = 1.0f;
     float v[8], w[8];
     if constexpr (MODE >= kNorm) {
-        float sum = 0.0f;
+        float sum[1] = {0.0f};
         for (int e = 8 * threadIdx.x; e < a.n; e += 8 * 1024) {
             load_chunk<MODE>(a, row, e, v);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum = fmaf(v[i], v[i], sum);
+            for (int i = 0; i < 8; ++i) sum[0] = fmaf(v[i], v[i], sum[0]);
         }
-        sum = across_waves<16>(wave_sum(sum), s_sum, [](float p, float q) { return p + q; });
-        f = norm_factor(sum, a);
+        sum[0] = wave_sum(sum[0]);
+        f = norm_factor(across_waves<16>(sum, s_sum, [](float p, float q) { return p + q; }), a);
     }
     auto scaled = [&](int e, bool raw) {
         load_chunk<MODE>(a, row, e, v);
@@ -304,15 +314,15 @@ __global__ __launch_bounds__(1024) void long_rows_kernel(const RowArgs a) {
     };
     Scale sc{0.0f, 1.0f, false, 0.0f};
     if (a.codes) {
-        uint32_t top = 0;
+        uint32_t top[1] = {0};
         for (int e = 8 * threadIdx.x; e < a.n; e += 8 * 1024) {
             scaled(e, false);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) top = max(top, magnitude(v[i]));
+            for (int i = 0; i < 8; ++i) top[0] = max(top[0], magnitude(v[i]));
         }
-        top = across_waves<16>(wave_max_u32(top), s_max,
-                               [](uint32_t p, uint32_t q) { return p > q ? p : q; });
-        sc = row_scale(top);
+        top[0] = wave_max_u32(top[0]);
+        sc = row_scale(across_waves<16>(top, s_max,
+                                        [](uint32_t p, uint32_t q) { return p > q ? p : q; }));
         if (threadIdx.x == 0) a.scales[row] = sc.scale;
     }
     for (int e = 8 * threadIdx.x; e < a.n; e += 8 * 1024) {

@@ -388,6 +388,7 @@ int af_qkv_rope_append(const void* x, const uint8_t* w_qkv, const void* scales, 
  * gets codes 0 and scale NaN: what is computed from it is NaN.
  * codes: row i at codes + i * codes_stride (bytes past n of a row are left as
  * they are), any alignment; scales: [m]. Every row is n elements, n <= 2^30.
+ * A row's outputs have the same bits whatever m and the other rows are.
  * Outputs overlap no input and no other output unless said so.
  *
  * af_quantize_rows: v = x, fp16 rows x_stride elements apart (attention's

@@ -322,6 +322,33 @@ def test_w8a8_gemm(gpu, m, n, k, dtype, bias, pad):
     assert np.all(err <= gemm_bound(p, y, dtype)), (err - gemm_bound(p, y, dtype)).max()
 
 
+@pytest.mark.parametrize("n", [1000, 4096, 4104, 5120, 7168, 8192, 12000, 40000])
+@pytest.mark.parametrize("res", [None, np.float16, np.float32])
+def test_rows_do_not_depend_on_their_number(gpu, n, res):
+    """A token's norm, codes and scale have the same bits alone and in any batch."""
+    say(f"row bits n={n} residual {res}")
+    m = 1100
+    r = np.random.default_rng(n)
+    x = r.standard_normal((m, n)).astype(np.float16)
+    residual = None if res is None else (3.0 * r.standard_normal((m, n))).astype(res)
+    w = up((1.0 + 0.2 * r.standard_normal(n)).astype(np.float32))
+    kinds = {}
+    for rows in (m, 600, 40, 1):
+        xr, c = Rows(np.float16, rows, n, n, 0, x[:rows]), Rows(np.int8, rows, n, n)
+        s, nr = Rows(np.float32, rows, 1, 1), Rows(np.float16, rows, n, n)
+        kw = {}
+        if res is not None:
+            rr = Rows(res, rows, n, n, 0, residual[:rows])
+            kw = dict(residual=rr.ptr, residual_out=rr.ptr, residual_stride=n,
+                      residual_dtype=AF_FP32 if res == np.float32 else AF_FP16)
+        kv.launch_rmsnorm_quantize(xr.ptr, n, w, 1e-5, rows, n, codes=c.ptr, codes_stride=n,
+                                   scales=s.ptr, normed=nr.ptr, normed_stride=n, **kw)
+        kinds[rows] = c.get(), s.get(), nr.get()
+    for rows in (600, 40, 1):
+        for whole, got in zip(kinds[m], kinds[rows]):
+            assert np.array_equal(whole[:rows], got), rows
+
+
 # Every form of the product, by its rule on a device of 256 CUs: one token in pairs of rows, the
 # tiles in the order of the table, with partial steps and tiles; for 256 x 256 tiles launches
 # of 1 to 13 steps, whole and partial, with one tile for some workgroups and two for others.
