@@ -349,6 +349,22 @@ def test_rows_do_not_depend_on_their_number(gpu, n, res):
             assert np.array_equal(whole[:rows], got), rows
 
 
+@pytest.mark.parametrize("n", [1000, 5120, 7168, 8192, 12000, 40000])
+def test_silu_rows_do_not_depend_on_their_number(gpu, n):
+    say(f"silu row bits n={n}")
+    m = 1100
+    x = (3.0 * np.random.default_rng(n).standard_normal((m, 2 * n))).astype(np.float16)
+    kinds = {}
+    for rows in (m, 600, 40, 1):
+        xr = Rows(np.float16, rows, 2 * n, 2 * n, 0, x[:rows])
+        c, s = Rows(np.int8, rows, n, n), Rows(np.float32, rows, 1, 1)
+        kv.launch_silu_mul_quantize(xr.ptr, xr.ptr + 2 * n, 2 * n, rows, n, c.ptr, n, s.ptr)
+        kinds[rows] = c.get(), s.get()
+    for rows in (600, 40, 1):
+        for whole, got in zip(kinds[m], kinds[rows]):
+            assert np.array_equal(whole[:rows], got), rows
+
+
 # Every form of the product, by its rule on a device of 256 CUs: one token in pairs of rows, the
 # tiles in the order of the table, with partial steps and tiles; for 256 x 256 tiles launches
 # of 1 to 13 steps, whole and partial, with one tile for some workgroups and two for others.
