@@ -284,6 +284,9 @@ void launch_rmsnorm_quantize(const __half* x, int64_t x_stride, View& residual, 
     if (!is_matrix(residual) || weight.dtype != DataType::FP32 || weight.num_dims != 1 ||
         weight.dims[0] != residual.dims[1] || weight.strides[0] != 1)
         throw std::runtime_error("launch_rmsnorm_quantize: residual [m, n], weight FP32 [n]");
+    // (the C ABI takes a null residual as the norm of x alone)
+    if (!residual.data_ptr && residual.dims[0] > 0)
+        throw std::runtime_error("launch_rmsnorm_quantize: null residual");
     check(af_rmsnorm_quantize(x, x_stride, residual.data_ptr, residual.data_ptr,
                               residual.strides[0], int(residual.dtype),
                               static_cast<const float*>(weight.data_ptr), eps,

@@ -168,7 +168,7 @@ void launch_silu_mul_quantize(const __half* gate, const __half* up, int64_t stri
                               int8_t* codes, int64_t codes_stride, float* scales,
                               hipStream_t stream);
 // af_rmsnorm_quantize: residual += x and its norm, as codes. residual [m, n] FP16 or
-// FP32 rows, updated in place; weight FP32 [n].
+// FP32 rows, updated in place (without memory it throws); weight FP32 [n].
 void launch_rmsnorm_quantize(const __half* x, int64_t x_stride, View& residual, const View& weight,
                              float eps, int8_t* codes, int64_t codes_stride, float* scales,
                              hipStream_t stream);

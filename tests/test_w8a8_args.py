@@ -185,3 +185,44 @@ def test_quantize_int8_refuses():
     for bad in (np.zeros(4), np.full((2, 3), np.nan), np.array([[1.0, np.inf]])):
         with pytest.raises(ValueError):
             weights.quantize_int8(bad)
+
+
+def test_cpp_norm_refuses_a_null_residual(tmp_path):
+    """The C++ norm adds into its residual: a View without memory is refused (the C ABI takes a null
+    residual as the norm of x alone), unless it has no rows."""
+    src = tmp_path / "t.cpp"
+    src.write_text(r'''
+#include <cstdio>
+#include <stdexcept>
+#include "ops/kernel.h"
+static const char* text(View res) {
+    static char said[256];
+    char* fake = reinterpret_cast<char*>(0x10000);
+    View w = create_contiguous_view(fake, DataType::FP32, {64});
+    std::snprintf(said, sizeof said, "nothing");
+    try {
+        launch_rmsnorm_quantize(reinterpret_cast<__half*>(fake), 64, res, w, 1e-5f,
+                                reinterpret_cast<int8_t*>(fake), 64, reinterpret_cast<float*>(fake), nullptr);
+    } catch (const std::runtime_error& e) {
+        std::snprintf(said, sizeof said, "%s", e.what());
+    }
+    return said;
+}
+int main() {
+    std::puts(text(create_contiguous_view(nullptr, DataType::FP32, {4, 64})));
+    std::puts(text(create_contiguous_view(nullptr, DataType::FP16, {4, 64})));
+    std::puts(text(create_contiguous_view(nullptr, DataType::FP16, {0, 64})));
+}
+''')
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    lib = os.path.dirname(atomflow_amd.LIB_PATH)
+    exe = tmp_path / "t"
+    subprocess.run(["g++", "-std=c++17", "-O1", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include", "-I",
+                    os.path.join(root, "include"), str(src), "-L", lib, "-latomflow_kv",
+                    "-L/opt/rocm/lib", "-lamdhip64", f"-Wl,-rpath,{lib}:/opt/rocm/lib", "-o", str(exe)],
+                   check=True)
+    # (no device is shown to the program: a call that passes the checks ends in the runtime's error)
+    env = dict(os.environ, HIP_VISIBLE_DEVICES="-1")
+    r = subprocess.run([str(exe)], capture_output=True, text=True, env=env)
+    said = r.stdout.split("\n")
+    assert r.returncode == 0 and all("null residual" in s for s in said[:2]) and said[2] == "nothing", r
