@@ -130,6 +130,30 @@ def test_quantize_rows_halves(gpu, m, n):
     assert np.array_equal(c.get(), exact_codes(x))
 
 
+@pytest.mark.parametrize("m,n", [(511, 5120), (512, 4097), (600, 5120), (520, 8190), (1100, 8192)])
+def test_quantize_rows_halves_of_large_batches(gpu, m, n):
+    """Rows of 4097 to 8192 elements: 1024 threads each up to twice the device's CUs (511 rows), 512
+    with two chunks each from there on, the form of a large prompt's attention output."""
+    test_quantize_rows_halves(gpu, m, n)
+
+
+@pytest.mark.parametrize("n", [1000, 4096, 4104, 5120, 7168, 8192, 12000, 40000])
+def test_plain_rows_do_not_depend_on_their_number(gpu, n):
+    say(f"plain row bits n={n}")
+    m = 1100
+    x = odd_rows(activations(m, n, n))[::-1]  # (the odd rows in every batch of 40)
+    kinds = {}
+    for rows in (m, 600, 40, 1):
+        xr = Rows(np.float16, rows, n, n, 0, x[:rows])
+        c, s = Rows(np.int8, rows, n, n), Rows(np.float32, rows, 1, 1)
+        kv.launch_quantize_rows(xr.ptr, n, rows, n, c.ptr, n, s.ptr)
+        kinds[rows] = c.get(), s.get()
+    check_codes(kinds[m][0], kinds[m][1][:, 0], x.astype(np.float64), 0.0, f"n={n}")
+    for rows in (600, 40, 1):
+        for whole, got in zip(kinds[m], kinds[rows]):
+            assert whole[:rows].tobytes() == got.tobytes(), rows
+
+
 @pytest.mark.parametrize("n", WIDTHS)
 @pytest.mark.parametrize("m,off,fused", [(1, 0, True), (9, 1, False), (33, 0, True)])
 def test_silu_mul_quantize(gpu, n, m, off, fused):
