@@ -69,6 +69,7 @@ PROTOTYPES = {
     "af_silu_mul_quantize": (I, [P, P, I64, I, I, P, I64, P, P]),
     "af_rmsnorm_quantize": (I, [P, I64, P, P, I64, I, P, F, I, I, P, I64, P, P, I64, P]),
     "af_w8a8_gemm": (I, [P, I64, P, I, P, I64, P, P, P, I64, I, I, I, P]),
+    "af_w8a8_gemm_form": (I, [I, I, I, P]),
     "af_prefill_rope_append": (I, [P, I, P, P, P, P, I, P, I, I, I, I, P, P]),
     "af_prefill_attention": (I, [P, I, P, P, P, I, I, I, I, I, I, I, I, P]),
     "af_tiled_attention": (I, [P, P, P, P, I, I, I, I, I, P]),

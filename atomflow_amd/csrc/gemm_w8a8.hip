@@ -736,13 +736,15 @@ void launch_row(const W8A8Args& a, hipStream_t s) {
                        0, s, a);
 }
 
+// Weights that one row of tiles (mb) reads are streamed, as the FP8 GEMV streams its own: those
+// under 12 MB may stay in the caches from one launch to the next.
+bool streams_weights(int mb, int n, int k) { return mb == 1 && int64_t(n) * k > 12 << 20; }
+
 template <typename Y, int S, int BM, int BN, int WR, int WC, int KS, int ST, int WGS>
 void launch_tiled(const W8A8Args& a, hipStream_t s) {
     const int mb = (a.m + BM - 1) / BM, tiles = mb * ((a.n + BN - 1) / BN);
     W8A8Args b = a;
-    // Weights that one row of tiles reads are streamed, as the FP8 GEMV streams its own: those
-    // under 12 MB may stay in the caches from one launch to the next.
-    b.stream_w = mb == 1 && int64_t(a.n) * a.k > 12 << 20;
+    b.stream_w = streams_weights(mb, a.n, a.k);
     hipLaunchKernelGGL((w8a8_tiled_kernel<Y, S, BM, BN, WR, WC, KS, ST, WGS>), dim3(tiles),
                        dim3(64 * WR * WC * KS), 0, s, b);
 }
@@ -791,11 +793,10 @@ constexpr TileCost kTileCost[kForms] = {
     {32, 256, 1, 2, 1.3309f, 2.1394f, 0.4646f, 0.1685f, 0.1281f, 0.0776f}
 };
 
-int pick_form(const W8A8Args& a) {
+int pick_form(unsigned m, unsigned n, unsigned k) {
     // (called for every launch: constant tile sizes, 32-bit arithmetic; tiles are below 2^29)
     const unsigned cus = unsigned(device_compute_units());
-    const unsigned m = unsigned(a.m), n = unsigned(a.n), k = unsigned(a.k);
-    const float weights = float(a.n) * float(a.k) * 1e-6f;  // MB
+    const float weights = float(int(n)) * float(int(k)) * 1e-6f;  // MB
     int best = 0;
     float best_cost = 0.0f;
 #pragma clang loop unroll(full)
@@ -816,13 +817,16 @@ int pick_form(const W8A8Args& a) {
     return best;
 }
 
+// One token: rows of one pass (four 1 KB chunks) each to a wave; longer ones in pairs. (us,
+// one row / two per wave: 6144 x 4096 5.8 / 5.9, 28672 x 4096 18.2 / 18.6, 4096 x 14336
+// 11.2 / 10.8; the best tiles 6.7, 20.9 and 11.5.)
+bool row_pairs(int k) { return k > 4096; }
+
 template <typename Y>
 void launch_w8a8(const W8A8Args& a, hipStream_t s) {
-    // One token: rows of one pass (four 1 KB chunks) each to a wave; longer ones in pairs. (us,
-    // one row / two per wave: 6144 x 4096 5.8 / 5.9, 28672 x 4096 18.2 / 18.6, 4096 x 14336
-    // 11.2 / 10.8; the best tiles 6.7, 20.9 and 11.5.)
-    if (a.m == 1) return a.k <= 4096 ? launch_row<Y, 1, 4>(a, s) : launch_row<Y, 2, 4>(a, s);
-    switch (pick_form(a)) {
+    if (a.m == 1)
+        return row_pairs(a.k) ? launch_row<Y, 2, 4>(a, s) : launch_row<Y, 1, 4>(a, s);
+    switch (pick_form(a.m, a.n, a.k)) {
         case k16x16k8: return launch_tiled<Y, 16, 16, 16, 1, 1, 8, 4, 1>(a, s);
         case k16x32k4: return launch_tiled<Y, 16, 16, 32, 1, 1, 4, 3, 2>(a, s);
         case k32x32k4: return launch_tiled<Y, 32, 32, 32, 1, 1, 4, 4, 1>(a, s);
@@ -844,6 +848,12 @@ void launch_w8a8(const W8A8Args& a, hipStream_t s) {
 
 bool aligned(const void* p, size_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 
+// Sums below 2^31 (2^14 k), and a launch of fewer than 2^32 threads.
+bool supported_sizes(int m, int n, int k) {
+    return k % 16 == 0 && k <= 131056 && m <= 1 << 25 && n <= 1 << 25 &&
+           int64_t(m) * n <= int64_t(1) << 36;
+}
+
 }  // namespace
 }  // namespace af
 
@@ -856,7 +866,7 @@ extern "C" int af_w8a8_gemm(const int8_t* x, int64_t x_stride, const float* x_sc
     if (!x || !x_scales || !weight || !w_scales || !y || m < 0 || n <= 0 || k <= 0)
         return AF_ERR_INVALID_ARG;
     if (y_dtype != AF_FP16 && y_dtype != AF_FP32) return AF_ERR_UNSUPPORTED;
-    if (k % 16 || k > 131056) return AF_ERR_UNSUPPORTED;  // 2^14 k < 2^31
+    if (!supported_sizes(m, n, k)) return AF_ERR_UNSUPPORTED;
     if (x_stride < k || w_stride < k || x_stride % 16 || w_stride % 16 || y_stride < n)
         return AF_ERR_INVALID_ARG;
     // 32-bit lane offsets within a tile's rows
@@ -864,8 +874,6 @@ extern "C" int af_w8a8_gemm(const int8_t* x, int64_t x_stride, const float* x_sc
     if (!aligned(x, 16) || !aligned(weight, 16) || !aligned(x_scales, 4) || !aligned(w_scales, 4) ||
         !aligned(bias, 4) || !aligned(y, y_dtype == AF_FP32 ? 4 : 2))
         return AF_ERR_INVALID_ARG;
-    // a launch has fewer than 2^32 threads
-    if (m > 1 << 25 || n > 1 << 25 || int64_t(m) * n > int64_t(1) << 36) return AF_ERR_UNSUPPORTED;
     if (m == 0) return AF_OK;
     W8A8Args a{};
     a.x = x;
@@ -884,5 +892,21 @@ extern "C" int af_w8a8_gemm(const int8_t* x, int64_t x_stride, const float* x_sc
     if (y_dtype == AF_FP32) launch_w8a8<float>(a, s);
     else launch_w8a8<uint16_t>(a, s);
     AF_TRY_LAUNCH();
+    return AF_OK;
+}
+
+extern "C" int af_w8a8_gemm_form(int m, int n, int k, int32_t* form) {
+    if (!form || m <= 0 || n <= 0 || k <= 0) return AF_ERR_INVALID_ARG;
+    if (!supported_sizes(m, n, k)) return AF_ERR_UNSUPPORTED;
+    if (m == 1) {
+        const int32_t row[5] = {1, row_pairs(k) ? 2 : 1, 1, 0, 1};
+        std::copy(row, row + 5, form);
+        return AF_OK;
+    }
+    const int i = pick_form(m, n, k);
+    const TileCost& c = kTileCost[i];
+    const bool streams = i != k256x256 && streams_weights((m + c.bm - 1) / c.bm, n, k);
+    const int32_t tile[5] = {c.bm, c.bn, c.ks, c.wgs, streams};
+    std::copy(tile, tile + 5, form);
     return AF_OK;
 }

@@ -128,6 +128,14 @@ def launch_w8a8_gemm(x, x_stride, x_scales, m, weight, w_stride, w_scales, y, y_
           "launch_w8a8_gemm")
 
 
+def w8a8_gemm_form(m, n, k):
+    """The kernel that launch_w8a8_gemm takes for these sizes: (tokens of a tile, weight rows of a
+    tile, parts of K, workgroups per CU, weights streamed)."""
+    form = (ctypes.c_int32 * 5)()
+    check(lib().af_w8a8_gemm_form(m, n, k, form), "w8a8_gemm_form")
+    return (*form[:4], bool(form[4]))
+
+
 # ---- prefill (multi-token append, causal attention over a prompt chunk) -----
 def launch_prefill_rope_append(qkv_out, n, k_cache, v_cache, cos_table, sin_table, p0, max_seq,
                                n_q_heads, n_kv_heads, head_dim, d_p0=None, d_status=None,
@@ -689,6 +697,7 @@ __all__ = [
     "launch_cached_attention_ex", "launch_decode_attention_fused", "launch_paged_attention",
     "launch_paged_decode_fused", "launch_paged_rope_append", "launch_qkv_rope_append",
     "launch_quantize_rows", "launch_rmsnorm_quantize", "launch_silu_mul_quantize", "launch_w8a8_gemm",
+    "w8a8_gemm_form",
     "launch_w8a16_gemv", "launch_prefill_rope_append", "launch_prefill_attention",
     "launch_tiled_attention_kernel", "launch_paged_prefill_attention", "Scheduler",
     "launch_paged_prefill_attention_batched", "prefill_tile_map",

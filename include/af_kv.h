@@ -431,6 +431,13 @@ int af_rmsnorm_quantize(const void* x, int64_t x_stride, const void* residual, v
 int af_w8a8_gemm(const int8_t* x, int64_t x_stride, const float* x_scales, int m,
                  const int8_t* weight, int64_t w_stride, const float* w_scales, const float* bias,
                  void* y, int64_t y_stride, int y_dtype, int n, int k, af_stream_t stream);
+/* Which kernel af_w8a8_gemm takes for these sizes on the current device (a host
+ * without one: for 256 CUs, MI355X's), host-only: form[5] = tokens and weight
+ * rows of a tile, parts of K in a workgroup, workgroups per CU, and 1 where each
+ * weight is read by one workgroup, non-temporally, from a k of the workgroup's
+ * own on (one row of tiles, more than 12 MB of weights). One token: 1 and the
+ * weight rows of a wave, 1, 0, 1. Every form gives the same bits. m >= 1. */
+int af_w8a8_gemm_form(int m, int n, int k, int32_t* form);
 
 /* ======================================================================== */
 /* b2. Prefill: multi-token append and causal attention over a prompt chunk */

@@ -437,6 +437,37 @@ def test_w8a8_gemm_wide(gpu, m, n, k):
     check_product(m, n, k, np.float32 if k % 32 else np.float16, n % 2 == 1, m % 2)
 
 
+# Tiled forms (tokens and weight rows of a tile, parts of K, workgroups per CU) whose one row of
+# tiles streams the weights, each workgroup from a k of its own on: loops longer than the stages,
+# loops of the stages' number and fewer, and a layer's projections. Partial steps and tiles.
+# (That each shape takes its form, and the lists together every form, is asserted on the host.)
+STREAMED = {
+    (16, 16, 8, 1): [(2, 2194, 5808), (2, 3131, 4080)],
+    (16, 32, 4, 2): [(2, 6071, 2080), (2, 9150, 1376), (16, 6144, 4096)],
+    (32, 32, 4, 1): [(18, 4526, 2800), (17, 7919, 1600)],
+    (32, 64, 2, 2): [(17, 8374, 1504), (2, 16784, 752), (8, 28672, 4096)],
+    (64, 32, 4, 1): [(35, 5550, 2320)],
+    (64, 64, 1, 2): [(34, 19227, 656), (33, 31696, 400)],
+    (64, 64, 2, 1): [(33, 8837, 1440), (33, 13769, 928)],
+    (128, 64, 2, 1): [(97, 10120, 1264)],
+    (128, 96, 1, 1): [(65, 16475, 1680)],
+    (128, 128, 1, 1): [(65, 22560, 560)],
+    (192, 128, 1, 1): [(130, 21869, 576), (130, 88084, 144)],
+    (192, 256, 1, 1): [(129, 38295, 400), (129, 112474, 112)],
+    (64, 128, 1, 2): [(2, 33463, 528), (33, 65625, 192), (45, 28672, 4096)],
+    (128, 128, 1, 2): [(98, 32921, 400), (66, 52453, 240)],
+    (32, 256, 1, 2): [(4, 49953, 400), (2, 79077, 160)],
+}
+# Several rows of tiles: a layer's projection, and the form that the lists above lack so.
+UNSTREAMED = [(32, 4096, 14336), (6435, 129, 1488)]
+
+
+@pytest.mark.parametrize("m,n,k", [q for shapes in STREAMED.values() for q in shapes] + UNSTREAMED)
+@pytest.mark.parametrize("dtype,bias,pad", [(np.float16, True, 1), (np.float32, False, 0)])
+def test_w8a8_gemm_streamed(gpu, m, n, k, dtype, bias, pad):
+    say(f"w8a8 streamed m={m} n={n} k={k} {np.dtype(dtype).name} {kv.w8a8_gemm_form(m, n, k)}")
+    check_product(m, n, k, dtype, bias, pad)
+
 @pytest.mark.parametrize("m,n", [(1, 1), (20, 3), (70, 40), (300, 129)])
 def test_w8a8_gemm_largest_sums(gpu, m, n):
     """The longest k with every code -128: 2^14 * 131056 just fits 32 bits."""

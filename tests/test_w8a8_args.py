@@ -226,3 +226,43 @@ int main() {
     r = subprocess.run([str(exe)], capture_output=True, text=True, env=env)
     said = r.stdout.split("\n")
     assert r.returncode == 0 and all("null residual" in s for s in said[:2]) and said[2] == "nothing", r
+
+
+def test_product_shapes_reach_every_form():
+    """The shapes that the GPU tests of the product run, by its rule on a device of 256 CUs (what a
+    host without a device assumes): every form that sizes drawn at random reach is among them, streamed
+    and not, and none of these launches passes 2^32 threads."""
+    import test_gpu_w8a8 as shapes
+
+    for form, cases in shapes.STREAMED.items():
+        for q in cases:
+            assert kv.w8a8_gemm_form(*q) == (*form, True), q
+    lists = shapes.SHAPES + shapes.FORMS + shapes.WIDE + shapes.UNSTREAMED
+    covered = {kv.w8a8_gemm_form(*q) for q in lists + sum(shapes.STREAMED.values(), [])}
+    tiles = {f[:4] for f in covered if f[0] > 1 and f[:2] != (256, 256)}
+    assert tiles == set(shapes.STREAMED)
+    r = np.random.default_rng(1)
+    for top_m, top_n in ((3, 18), (6, 14), (8, 18), (13, 15), (25, 25)):
+        m = np.exp2(r.uniform(0, top_m, 20000)).astype(int)
+        n = np.exp2(r.uniform(0, top_n, 20000)).astype(int)
+        k = 16 * np.exp2(r.uniform(0, 12.9, 20000)).astype(int)
+        for q in zip(m.tolist(), n.tolist(), k.tolist()):
+            if q[0] * q[1] > 1 << 36:
+                continue
+            form = kv.w8a8_gemm_form(*q)
+            assert form in covered, (q, form)
+            assert form[0] == 1 or -(-q[0] // form[0]) * -(-q[1] // form[1]) * 512 < 1 << 32, (q, form)
+
+
+def test_product_form_refusals():
+    form = np.zeros(5, np.int32)
+    f = atomflow_amd.lib().af_w8a8_gemm_form
+    for bad in ((0, 8, 16), (-1, 8, 16), (4, 0, 16), (4, 8, 0)):
+        assert f(*bad, form.ctypes.data) == BAD
+    assert f(4, 8, 16, None) == BAD
+    for no in ((4, 8, 40), (4, 8, 131072), ((1 << 25) + 1, 8, 16), (4, (1 << 25) + 1, 16),
+               (1 << 20, 1 << 17, 16)):
+        assert f(*no, form.ctypes.data) == NOT
+    assert not form.any()
+    assert kv.w8a8_gemm_form(1, 64, 4096) == (1, 1, 1, 0, True)
+    assert kv.w8a8_gemm_form(1, 64, 4112) == (1, 2, 1, 0, True)
