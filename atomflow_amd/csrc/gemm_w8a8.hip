@@ -5,12 +5,13 @@
 // One scale per token and one per output channel factor out of the sum, so the matrix
 // cores add whole products of codes in 32 bits. These sums are exact (|sum| <= 2^14 k <
 // 2^31 for k <= 131056): every order, split and tile gives the same bits, and a token's
-// row does not depend on the launch it is in. The sum becomes fp32 (its one rounding
-// before the result's, 2^-25 relative at most) and takes the scales and the bias there.
+// row does not depend on the launch it is in. The sum becomes fp32 and takes the scales and
+// the bias there: its conversion and its product with sx round by 2^-24 at most each, before
+// the rounding of the multiply-add with sw and the bias and the one to the result's type.
 //
 // Three kernels: one token (w8a8_row_kernel) and the tiles of few tokens (w8a8_tiled_kernel)
-// are bound by the weights' stream, tiles in between by what a CU loads from L2, large
-// launches (w8a8_wide_kernel) by the card's power. pick_form chooses by measured cost.
+// are bound by the weights' stream, large launches (w8a8_wide_kernel) by the card's power;
+// launches in between reach no ceiling. pick_form chooses by measured cost.
 #include <algorithm>
 
 #include "af_common.h"
@@ -59,9 +60,9 @@ __device__ __forceinline__ uint32_t half_pair(float lo, float hi) {
 // contiguous 1 KB chunks, 16 bytes per lane, non-temporally (each weight byte is read once
 // by the launch); a chunk of the token's codes is loaded once for the R rows. All loads of a
 // pass of U chunks go out before any is used. v_dot4_i32_i8 adds four products a lane, and
-// the lanes' sums meet by cross-lane adds. Bound by HBM: 28672 x 4096 in 18.2 us, 128256 x
-// 4096 in 74, 7.1 TB/s (a 16 x 16 x 64 matrix-core product fed with 64-byte pieces of 16 rows
-// took 25.6 and 123). Two tokens are no faster here than on the tiles.
+// the lanes' sums meet by cross-lane adds. Bound by HBM: 28672 x 4096 in 18.7 us (6.3 TB/s, the
+// launch in it), 128256 x 4096 in 76 (6.9; a 16 x 16 x 64 matrix-core product fed with 64-byte
+// pieces of 16 rows took 25.6 and 123). Two tokens are no faster here than on the tiles.
 constexpr int kRowWaves = 4;
 
 __device__ __forceinline__ int wave_sum_i32(int v) {
@@ -132,12 +133,14 @@ __global__ __launch_bounds__(64 * kRowWaves) void w8a8_row_kernel(const W8A8Args
 // stage's first operands are read under the last products of this one. A part of one wave
 // needs no barrier: it loads what it reads.
 //
-// What bounds it, between a few dozen and a few hundred tokens, is the loads: 8 rows of 128
-// bytes an instruction reach 98 GB/s per CU from L2 (1 KB pieces 145), and HBM's latency. 513
-// x 4096 x 14336 runs in 60 us (weights from HBM) with the matrix cores busy a quarter of the
-// time; stages twice as many or as long, operands a whole step ahead, waves of 64 x 64 and 64 x
-// 96 (which read a third less from LDS), and a wave that touches the weights' lines early gave
-// nothing or cost time.
+// Between a few dozen and a few hundred tokens it reaches no ceiling, and what holds it is not
+// established. 513 x 4096 x 14336 runs in 60 us (weights from HBM): the matrix cores are busy a
+// quarter of the time, HBM moves 1.2 TB/s, and each of the 215 workgroups loads 53 GB/s, where
+// loads of 8 rows of 128 bytes an instruction reach 98 per CU from L2 (1 KB pieces 145). All
+// workgroups ask for the same k of rows a fixed stride apart at a time; where one row of tiles
+// reads the weights that alone cost a third (the turned start, below). Stages twice as many or
+// as long, operands a whole step ahead, waves of 64 x 64 and 64 x 96 (which read a third less
+// from LDS), and a wave that touches the weights' lines early gave nothing or cost time.
 constexpr int kStep = 128;
 
 // lds_dma16 of a wave-uniform base and lane offsets, non-temporal.
@@ -455,9 +458,9 @@ w8a8_tiled_kernel(const W8A8Args a) {
 
 // ---- 256 x 256 tiles --------------------------------------------------------------
 // Large launches: a workgroup of eight waves (128 x 64 of y each, two per SIMD) per CU, which
-// walks its tiles. What bounds it is the card's power: the matrix cores are busy two thirds
-// of the cycles at 1.7 GHz (a form that kept them busy half of the cycles ran at 1.9 GHz), so
-// the rest is kept off them: 32x32x32 products, 128-byte rows from L2, no LDS conflict.
+// walks its tiles. What bounds it is the card's power: the matrix cores are busy 71 % of the
+// cycles at 1.5 GHz (a form that kept them busy half of the cycles ran at 1.9 GHz), so the
+// rest is kept off them: 32x32x32 products, 128-byte rows from L2, no LDS conflict.
 //
 // LDS is a ring of five 32 KB slots: load L of the sequence x0, w0, x1, w1, .. (the step's 256
 // token rows, its 256 weight rows) takes slot L % 5. One barrier per step, before its last
@@ -465,9 +468,9 @@ w8a8_tiled_kernel(const W8A8Args a) {
 // for w of the next step but one and x of the one after, a few 1 KB loads between two products
 // each; x then has a step and a half to arrive, w one and a quarter. The sequence runs on
 // across tiles: the next tile's first loads are issued before this tile's output, which goes
-// through the two slots that its last step leaves (the products of 8192 x 28672 x 4096 took
-// 872 us with one workgroup per tile and stages of whole steps, 811 like this; a library
-// product of the same integers 908).
+// through the two slots that its last step leaves. 8192 x 28672 x 4096 takes 786 us (a library
+// product of the same integers 908; this kernel's first form 811, where one workgroup per
+// tile with stages of whole steps took 872).
 template <typename Y, int MT, int NT>
 __device__ __forceinline__ void store_wide(const W8A8Args& a, int t0, int n0, int lane, char* s,
                                            const int16v_t (&acc)[MT][NT]) {
@@ -763,7 +766,8 @@ void launch_wide(const W8A8Args& a, hipStream_t s) {
 // the busiest CUs `share` and of the average CU `spread` (us); a launch `fixed` besides, and
 // `stream` per MB of weights. Small tiles with several parts of K at a time fill the device
 // when tokens or rows are few, large ones read the least and keep the matrix cores busiest.
-// The rule picks a form within 1.5 % of the best measured one on average (23 % at most).
+// The rule's form takes 1.4 % more than the best measured one on average, 23 % at most, of the
+// launches that the costs were fitted to.
 struct TileCost {
     int bm, bn, ks, wgs;
     float fixed, round, step, share, spread, stream;
