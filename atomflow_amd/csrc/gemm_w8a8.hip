@@ -800,7 +800,7 @@ constexpr TileCost kTileCost[kForms] = {
 int pick_form(unsigned m, unsigned n, unsigned k) {
     // (called for every launch: constant tile sizes, 32-bit arithmetic; tiles are below 2^29)
     const unsigned cus = unsigned(device_compute_units());
-    const float weights = float(int(n)) * float(int(k)) * 1e-6f;  // MB
+    const float weights = float(n) * float(k) * 1e-6f;  // MB
     int best = 0;
     float best_cost = 0.0f;
 #pragma clang loop unroll(full)
