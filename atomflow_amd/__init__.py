@@ -34,6 +34,8 @@ AF_KV_FP8_E4M3 = 3
 AF_KV_POOL_SHARED_BLOCKS = 1
 AF_FP32 = 0
 AF_FP16 = 1
+AF_ROPE_HALF = 0
+AF_ROPE_INTERLEAVED = 1
 
 
 class AfError(RuntimeError):

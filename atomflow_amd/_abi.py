@@ -31,6 +31,45 @@ class KvPool(ctypes.Structure):
 
 PPOOL = ctypes.POINTER(KvPool)
 
+
+class RopeScaling(ctypes.Structure):
+    """af_rope_scaling (include/af_kv.h)."""
+
+    _fields_ = [
+        ("kind", I32),
+        ("original_max_pos", I32),
+        ("base", ctypes.c_double),
+        ("factor", ctypes.c_double),
+        ("low_freq_factor", ctypes.c_double),
+        ("high_freq_factor", ctypes.c_double),
+        ("beta_fast", ctypes.c_double),
+        ("beta_slow", ctypes.c_double),
+        ("attention_factor", ctypes.c_double),
+    ]
+
+
+LORA_MAX_SLICES = 4
+
+
+class Lora(ctypes.Structure):
+    """af_lora (include/af_kv.h)."""
+
+    _fields_ = [
+        ("a", P),
+        ("b", P),
+        ("ranks", P),
+        ("scales", P),
+        ("n_adapters", I32),
+        ("max_rank", I32),
+        ("n_slices", I32),
+        ("k", I32),
+        ("n", I32),
+        ("slice_end", I32 * LORA_MAX_SLICES),
+    ]
+
+
+PLORA = ctypes.POINTER(Lora)
+
 PROTOTYPES = {
     # af_kv.h
     "af_status_string": (ctypes.c_char_p, [I]),
@@ -59,6 +98,13 @@ PROTOTYPES = {
                                                 P, I, I, I, P, SZ, P]),
     "af_paged_gather": (I, [PPOOL, I, P, I, P, P, P]),
     "af_kv_copy_blocks": (I, [PPOOL, P, P, I, P]),
+    "af_rope_frequencies": (I, [ctypes.POINTER(RopeScaling), I, P, P]),
+    "af_rope_table_scaled": (I, [P, P, I64, I, I, P, ctypes.c_double, P]),
+    "af_rope_rows": (I, [P, I64, P, I64, I, P, I64, P, I64, I, I, I, I, I, I, P, P, I, P, I, P, P]),
+    "af_paged_rope_append_rows": (I, [P, I64, I, P, I64, I, PPOOL, I, P, P, I, I, P, P, I, P, P]),
+    "af_kv_compact": (I, [PPOOL, P, P, I, I, P, P, P, I, I, I, P, P, I, F, P, P]),
+    "af_lora_workspace_size": (SZ, [PLORA, I]),
+    "af_lora_add": (I, [P, I64, I, P, PLORA, P, I64, P, I64, I, P, SZ, P]),
     "af_fp8_quantize": (I, [P, P, SZ, F, P]),
     "af_w8a16_gemv": (I, [P, P, P, P, I, I, I, P]),
     "af_w8a16_gemm_batched": (I, [P, I64, I, P, P, P, I64, I, I, I, P]),
@@ -120,6 +166,7 @@ PROTOTYPES = {
     "af_bm_seq_extend": (I, [P, I, I, PI32, PI32, PI32]),
     "af_bm_seq_slot": (I64, [P, I, I]),
     "af_bm_plan_decode": (I, [P, P, I, P, P, P, I, PI32]),
+    "af_bm_plan_compact": (I, [P, P, I, P, P, P, P, I, P, P, P, PI32]),
     "af_bm_export_tables": (I, [P, P, I, P, I, P]),
     # af_runtime.h
     "af_rt_device_count": (I, [ctypes.POINTER(I)]),

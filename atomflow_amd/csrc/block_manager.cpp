@@ -3,6 +3,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <new>
 #include <string>
 
@@ -287,6 +288,80 @@ int BlockManager::plan_decode(const int* seqs, int n, AppendSlot* out) {
     return AF_OK;
 }
 
+int BlockManager::plan_compact(const int* seqs, int n, const int* keep, const int* keep_start,
+                               CompactPlan* out) {
+    if (!out || n < 0 || (n > 0 && (!seqs || !keep_start || keep_start[0] < 0)))
+        return AF_ERR_INVALID_ARG;
+    for (int i = 0; i < n; ++i)
+        if (!has_sequence(seqs[i])) return AF_ERR_BAD_SEQUENCE;
+    std::vector<int> sorted(seqs, seqs + n);
+    std::sort(sorted.begin(), sorted.end());
+    if (std::adjacent_find(sorted.begin(), sorted.end()) != sorted.end()) return AF_ERR_INVALID_ARG;
+
+    const int bs = cfg_.block_size;
+    // Others may read the block: at the plan's start, so that two forks of one launch both leave
+    // it alone, whichever of them drops its reference first.
+    auto shared = [&](int b) { return ref_[size_t(b)] > 1 || held_[size_t(b)] > 0; };
+    CompactPlan p;
+    p.start.push_back(0);
+    size_t fresh = 0;
+    for (int i = 0; i < n; ++i) {
+        const PageTable& t = tables_[size_t(seqs[i])];
+        const int len = seq_len(seqs[i]), count = keep_start[i + 1] - keep_start[i];
+        if (count < 0 || (count > 0 && !keep)) return AF_ERR_INVALID_ARG;
+        const int* rows = keep + keep_start[i];
+        int first = count;  // the first row that has to be written
+        for (int j = count - 1; j >= 0; --j) {
+            if (rows[j] < 0 || rows[j] >= len) return AF_ERR_OUT_OF_RANGE;
+            if (j > 0 && rows[j] <= rows[j - 1]) return AF_ERR_INVALID_ARG;
+            if (rows[j] != j) first = j;
+        }
+        // a block to be replaced takes its leading rows along
+        if (first < count && shared(t.block_ids[size_t(first / bs)])) first = first / bs * bs;
+        for (int b = first / bs; first < count && b <= (count - 1) / bs; ++b)
+            fresh += shared(t.block_ids[size_t(b)]);
+        p.first.push_back(first);
+        p.keep.insert(p.keep.end(), rows + first, rows + count);
+        p.start.push_back(int32_t(p.keep.size()));
+        p.max_rows = std::max(p.max_rows, count - first);
+        p.max_blocks = std::max(p.max_blocks, int(t.block_ids.size()));
+    }
+    if (fresh > free_list_.size()) return AF_ERR_POOL_EXHAUSTED;
+    p.max_blocks = std::max(p.max_blocks, 1);
+    p.src_tables.assign(size_t(n) * p.max_blocks, 0);
+    p.dst_tables.assign(size_t(n) * p.max_blocks, 0);
+
+    // New blocks first, from the list as it is: a block that this plan frees is still a source.
+    std::vector<int> dropped;
+    dropped.reserve(size_t(n) * p.max_blocks);
+    std::vector<uint8_t> replace(size_t(cfg_.total_blocks), 0);
+    for (int i = 0; i < n; ++i)
+        for (int b : tables_[size_t(seqs[i])].block_ids) replace[size_t(b)] = shared(b);
+    for (int i = 0; i < n; ++i) {
+        PageTable& t = tables_[size_t(seqs[i])];
+        std::copy(t.block_ids.begin(), t.block_ids.end(),
+                  p.src_tables.begin() + size_t(i) * p.max_blocks);
+        const int count = keep_start[i + 1] - keep_start[i];
+        const int blocks = (count + bs - 1) / bs;
+        if (p.first[size_t(i)] < count)
+            for (int b = p.first[size_t(i)] / bs; b < blocks; ++b) {
+                int& id = t.block_ids[size_t(b)];
+                if (!replace[size_t(id)]) continue;
+                dropped.push_back(id);
+                id = pop_free();
+            }
+        for (size_t b = size_t(blocks); b < t.block_ids.size(); ++b)
+            dropped.push_back(t.block_ids[b]);
+        t.block_ids.resize(size_t(blocks));
+        t.last_block_fill = count ? count - (blocks - 1) * bs : 0;
+        std::copy(t.block_ids.begin(), t.block_ids.end(),
+                  p.dst_tables.begin() + size_t(i) * p.max_blocks);
+    }
+    for (int b : dropped) (void)try_free_block(b);
+    *out = std::move(p);
+    return AF_OK;
+}
+
 }  // namespace atomflow::server
 
 // ============================================================================
@@ -294,6 +369,7 @@ int BlockManager::plan_decode(const int* seqs, int n, AppendSlot* out) {
 // ============================================================================
 using atomflow::server::AppendSlot;
 using atomflow::server::BlockManager;
+using atomflow::server::CompactPlan;
 using atomflow::server::CowCopy;
 using atomflow::server::PoolConfig;
 
@@ -447,6 +523,39 @@ extern "C" int af_bm_plan_decode(af_block_manager* bm, const int32_t* seqs, int 
     }
     *n_copies = nc;
     return nc > max_copies ? AF_ERR_OUT_OF_RANGE : AF_OK;
+}
+
+extern "C" int af_bm_plan_compact(af_block_manager* bm, const int32_t* seqs, int n,
+                                  const int32_t* keep, const int32_t* keep_start,
+                                  int32_t* src_tables, int32_t* dst_tables, int max_blocks,
+                                  int32_t* moved, int32_t* start, int32_t* first,
+                                  int32_t* max_rows) {
+    if (!bm || n < 0 || max_blocks <= 0 || !start || !max_rows ||
+        (n > 0 && (!seqs || !keep_start || !src_tables || !dst_tables || !first)))
+        return AF_ERR_INVALID_ARG;
+    for (int i = 0; i < n; ++i) {
+        if (!bm->bm.has_sequence(seqs[i])) return AF_ERR_BAD_SEQUENCE;
+        if (int(bm->bm.table(seqs[i]).block_ids.size()) > max_blocks) return AF_ERR_OUT_OF_RANGE;
+        if (keep_start[i + 1] > keep_start[i] && (!keep || !moved)) return AF_ERR_INVALID_ARG;
+    }
+    CompactPlan p;
+    try {
+        const int st = bm->bm.plan_compact(seqs, n, keep, keep_start, &p);
+        if (st) return st;
+    } catch (const std::exception&) {  // (thrown before anything has changed)
+        return int(hipErrorOutOfMemory);
+    }
+    for (int i = 0; i < n; ++i)
+        for (int b = 0; b < max_blocks; ++b) {
+            const bool in = b < p.max_blocks;
+            src_tables[size_t(i) * max_blocks + b] = in ? p.src_tables[size_t(i) * p.max_blocks + b] : 0;
+            dst_tables[size_t(i) * max_blocks + b] = in ? p.dst_tables[size_t(i) * p.max_blocks + b] : 0;
+        }
+    std::copy(p.keep.begin(), p.keep.end(), moved);
+    std::copy(p.start.begin(), p.start.end(), start);
+    std::copy(p.first.begin(), p.first.end(), first);
+    *max_rows = p.max_rows;
+    return AF_OK;
 }
 
 extern "C" int af_bm_export_tables(const af_block_manager* bm, const int32_t* seqs, int n,

@@ -41,6 +41,62 @@ def launch_rope(q, k, cos_cache, sin_cache, seq_len, kv_head_num, q_head_num, he
                         q_head_num, head_dim, _s(stream)), "launch_rope")
 
 
+# ---- a2': rotary positions in other forms ----------------------------------
+ROPE_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "bands": 3, "yarn": 4}
+
+
+def rope_frequencies(rot_dim, base=500000.0, scaling="none", factor=1.0, original_max_pos=0,
+                     low_freq_factor=1.0, high_freq_factor=4.0, beta_fast=32.0, beta_slow=1.0,
+                     attention_factor=0.0):
+    """(angles per position, float64 [rot_dim / 2], and the factor on cos and sin) of rotary
+    positions stretched by ``scaling``: "none", "linear", "ntk", "bands" or "yarn"."""
+    if scaling not in ROPE_SCALINGS:
+        raise ValueError(f"scaling {scaling!r}: one of {', '.join(ROPE_SCALINGS)}")
+    sc = _abi.RopeScaling(ROPE_SCALINGS[scaling], original_max_pos, base, factor, low_freq_factor,
+                          high_freq_factor, beta_fast, beta_slow, attention_factor)
+    freq = np.empty(max(rot_dim, 0) // 2, np.float64)
+    mult = ctypes.c_double()
+    check(lib().af_rope_frequencies(ctypes.byref(sc), rot_dim, freq.ctypes.data,
+                                    ctypes.byref(mult)), "rope_frequencies")
+    return freq, mult.value
+
+
+def build_rope_table_scaled(d_cos, d_sin, first_pos, n_rows, rot_dim, freq, factor=1.0,
+                            stream=None):
+    """Rows [first_pos, first_pos + n_rows) of the cos / sin table of ``freq`` (host, float64
+    [rot_dim / 2]), times ``factor``, in one launch."""
+    freq = np.ascontiguousarray(freq, np.float64)
+    if freq.shape != (rot_dim // 2,):
+        raise ValueError(f"freq has shape {freq.shape}, rot_dim {rot_dim} needs ({rot_dim // 2},)")
+    check(lib().af_rope_table_scaled(_p(d_cos), _p(d_sin), first_pos, n_rows, rot_dim,
+                                     freq.ctypes.data, factor, _s(stream)),
+          "build_rope_table_scaled")
+
+
+def launch_rope_rows(q, q_stride, q_out, q_out_stride, n_q_heads, k, k_stride, k_out, k_out_stride,
+                     n_k_heads, m, head_dim, rot_dim, layout, cos_table, sin_table, max_pos,
+                     positions=None, p0=0, inverse=False, d_status=None, stream=None):
+    """Rotary positions of m rows of Q and K (k None: Q alone), in place or out of place: the
+    first rot_dim elements of a head, in halves (AF_ROPE_HALF) or neighbours
+    (AF_ROPE_INTERLEAVED); ``inverse`` turns back."""
+    check(lib().af_rope_rows(_p(q), q_stride, _p(q_out), q_out_stride, n_q_heads, _p(k), k_stride,
+                             _p(k_out), k_out_stride, n_k_heads, m, head_dim, rot_dim, layout,
+                             1 if inverse else 0, _p(cos_table), _p(sin_table), max_pos,
+                             _p(positions), p0, _p(d_status), _s(stream)), "launch_rope_rows")
+
+
+def launch_paged_rope_append_rows(qkv, qkv_stride, m, q_out, q_out_stride, n_q_heads, pool, layer,
+                                  d_slots, d_positions, rot_dim, layout, cos_table, sin_table,
+                                  max_pos, d_status=None, stream=None):
+    """launch_paged_rope_append in these forms: Q turned into q_out, K (turned) and V into rows
+    d_slots of the pool (slot -1: not cached); qkv is only read."""
+    check(lib().af_paged_rope_append_rows(_p(qkv), qkv_stride, m, _p(q_out), q_out_stride,
+                                          n_q_heads, ctypes.byref(pool), layer, _p(d_slots),
+                                          _p(d_positions), rot_dim, layout, _p(cos_table),
+                                          _p(sin_table), max_pos, _p(d_status), _s(stream)),
+          "launch_paged_rope_append_rows")
+
+
 def launch_write_kv_cache(qkv_out, k_cache, v_cache, current_pos, q_dim, kv_dim, max_seq,
                           stream=None):
     check(lib().af_write_kv_cache(_p(qkv_out), _p(k_cache), _p(v_cache), current_pos, max_seq,
@@ -134,6 +190,35 @@ def w8a8_gemm_form(m, n, k):
     form = (ctypes.c_int32 * 5)()
     check(lib().af_w8a8_gemm_form(m, n, k, form), "w8a8_gemm_form")
     return (*form[:4], bool(form[4]))
+
+
+# ---- low-rank adapters beside a shared projection ----------------------------
+def make_lora(a, b, n_adapters, max_rank, k, slice_ends, ranks=None, scales=None):
+    """The adapters of one projection (af_lora): a fp16 [n_adapters, n_slices, max_rank, k], b
+    fp16 [n_adapters, n, max_rank]; slice_ends: where each part of a fused product's columns
+    ends (the last: n). The device arrays stay the caller's."""
+    ends = [int(e) for e in slice_ends]
+    if not 1 <= len(ends) <= _abi.LORA_MAX_SLICES:
+        raise ValueError(f"{len(ends)} slices: 1 to {_abi.LORA_MAX_SLICES}")
+    return _abi.Lora(_p(a), _p(b), _p(ranks), _p(scales), n_adapters, max_rank, len(ends), k,
+                     ends[-1], (ctypes.c_int32 * _abi.LORA_MAX_SLICES)(*ends))
+
+
+def lora_workspace_size(lora, m):
+    """Workspace bytes of launch_lora_add for up to m tokens."""
+    n = lib().af_lora_workspace_size(ctypes.byref(lora), m)
+    if n == 0:
+        raise AfError(-2, "lora_workspace_size")
+    return n
+
+
+def launch_lora_add(x, x_stride, m, ids, lora, y, y_stride, y_out, y_out_stride, workspace,
+                    workspace_bytes, y_dtype=AF_FP16, stream=None):
+    """y_out = y + scale * B (A x) with each token's adapter (ids: device int32 [m], -1 for
+    none); y_out may be y."""
+    check(lib().af_lora_add(_p(x), x_stride, m, _p(ids), ctypes.byref(lora), _p(y), y_stride,
+                            _p(y_out), y_out_stride, y_dtype, _p(workspace), workspace_bytes,
+                            _s(stream)), "launch_lora_add")
 
 
 # ---- prefill (multi-token append, causal attention over a prompt chunk) -----
@@ -413,6 +498,17 @@ def kv_copy_blocks(pool, d_copies, d_count, max_copies, stream=None):
                                   _s(stream)), "kv_copy_blocks")
 
 
+def kv_compact(pool, d_src_tables, d_dst_tables, max_blocks, n_seqs, d_keep, d_start, d_first,
+               max_rows, rot_dim=0, layout=0, cos_table=None, sin_table=None, max_pos=0,
+               table_factor=1.0, d_status=None, stream=None):
+    """Moves the kept rows of cached sequences up, every layer, K turned to the new positions
+    (rot_dim 0: as they are). Sequence s: logical row d_first[s] + i <- d_keep[d_start[s] + i]."""
+    check(lib().af_kv_compact(ctypes.byref(pool), _p(d_src_tables), _p(d_dst_tables), max_blocks,
+                              n_seqs, _p(d_keep), _p(d_start), _p(d_first), max_rows, rot_dim,
+                              layout, _p(cos_table), _p(sin_table), max_pos, table_factor,
+                              _p(d_status), _s(stream)), "kv_compact")
+
+
 def fp8_quantize(src_f16, dst, n, scale, stream=None):
     check(lib().af_fp8_quantize(_p(src_f16), _p(dst), n, scale, _s(stream)), "fp8_quantize")
 
@@ -535,6 +631,35 @@ class BlockManager:
         if r < 0:
             return r
         return slots, pos, copies[: nc.value].copy()
+
+    def plan_compact(self, seqs, keeps, max_blocks=None):
+        """Cuts each sequence to its logical rows ``keeps[i]`` (strictly increasing). Returns the
+        host arrays that kv_compact reads, as a dict (src_tables, dst_tables, keep, start,
+        first, max_rows; max_rows 0: nothing moves), or a negative status (nothing changed)."""
+        seqs = np.ascontiguousarray(seqs, np.int32)
+        n = len(seqs)
+        if len(keeps) != n:
+            raise ValueError(f"{n} sequences, {len(keeps)} lists of rows")
+        keeps = [np.asarray(k, np.int32).reshape(-1) for k in keeps]
+        start = np.zeros(n + 1, np.int32)
+        start[1:] = np.cumsum([len(k) for k in keeps])
+        keep = np.ascontiguousarray(np.concatenate(keeps + [np.zeros(1, np.int32)]))
+        if max_blocks is None:
+            counts = [lib().af_bm_seq_table(self.h, int(s), None, 0, None) for s in seqs]
+            max_blocks = max([1] + counts)
+        tables = np.zeros((2, n, max_blocks), np.int32)
+        moved = np.zeros(max(int(start[-1]), 1), np.int32)
+        first, at = np.zeros(n, np.int32), np.zeros(n + 1, np.int32)
+        most = ctypes.c_int32(0)
+        r = lib().af_bm_plan_compact(self.h, seqs.ctypes.data, n, keep.ctypes.data,
+                                     start.ctypes.data, tables[0].ctypes.data,
+                                     tables[1].ctypes.data, max_blocks, moved.ctypes.data,
+                                     at.ctypes.data, first.ctypes.data, ctypes.byref(most))
+        if r < 0:
+            return r
+        check(r, "plan_compact")
+        return {"src_tables": tables[0], "dst_tables": tables[1], "keep": moved[:at[-1]].copy(),
+                "start": at, "first": first, "max_rows": most.value}
 
     def export_tables(self, seqs, max_blocks):
         seqs = np.ascontiguousarray(seqs, np.int32)
@@ -697,7 +822,9 @@ __all__ = [
     "launch_cached_attention_ex", "launch_decode_attention_fused", "launch_paged_attention",
     "launch_paged_decode_fused", "launch_paged_rope_append", "launch_qkv_rope_append",
     "launch_quantize_rows", "launch_rmsnorm_quantize", "launch_silu_mul_quantize", "launch_w8a8_gemm",
-    "w8a8_gemm_form",
+    "w8a8_gemm_form", "build_rope_table_scaled", "kv_compact", "launch_lora_add",
+    "launch_paged_rope_append_rows", "launch_rope_rows", "lora_workspace_size", "make_lora",
+    "rope_frequencies",
     "launch_w8a16_gemv", "launch_prefill_rope_append", "launch_prefill_attention",
     "launch_tiled_attention_kernel", "launch_paged_prefill_attention", "Scheduler",
     "launch_paged_prefill_attention_batched", "prefill_tile_map",

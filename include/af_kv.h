@@ -225,6 +225,93 @@ int af_paged_rope_append(void* qkv_out, int batch, const af_kv_pool* pool, int l
                          const float* cos_table, const float* sin_table, int max_pos,
                          int n_q_heads, af_stream_t stream);
 
+/* ======================================================================== */
+/* a2'. Rotary positions in other forms                                      */
+/* ======================================================================== */
+/* The first rot_dim elements of a head turn (rot_dim even, 2 .. head_dim), the
+ * others stay as they are: pairs (d, d + rot_dim/2), as af_rope has them, or
+ * (2d, 2d + 1). */
+#define AF_ROPE_HALF 0
+#define AF_ROPE_INTERLEAVED 1
+
+/* How the angle per position of pair i, f_i = base^(-2i / rot_dim), is stretched for
+ * contexts longer than the trained one (original_max_pos positions):
+ *   NONE    f_i
+ *   LINEAR  f_i / factor
+ *   NTK     f_i of the base  base * factor^(rot_dim / (rot_dim - 2))
+ *   BANDS   by wavelength w = 2 pi / f_i: f_i where w < original_max_pos / high_freq_factor,
+ *           f_i / factor where w > original_max_pos / low_freq_factor, and between them
+ *           (1 - t) f_i / factor + t f_i,
+ *           t = (original_max_pos / w - low_freq_factor) / (high_freq_factor - low_freq_factor)
+ *   YARN    (1 - t) f_i + t f_i / factor, t = clamp((i - lo) / (hi - lo), 0, 1), between the
+ *           pairs that turn beta_fast and beta_slow times within original_max_pos:
+ *           lo = max(floor(d(beta_fast)), 0), hi = min(ceil(d(beta_slow)), rot_dim - 1),
+ *           d(b) = rot_dim ln(original_max_pos / (2 pi b)) / (2 ln base), hi - lo at least 0.001;
+ *           cos and sin are multiplied by 0.1 ln(factor) + 1.
+ * attention_factor, where it is not 0, replaces the kind's own factor on cos and sin (1 but
+ * for YARN). */
+#define AF_ROPE_SCALE_NONE 0
+#define AF_ROPE_SCALE_LINEAR 1
+#define AF_ROPE_SCALE_NTK 2
+#define AF_ROPE_SCALE_BANDS 3
+#define AF_ROPE_SCALE_YARN 4
+typedef struct af_rope_scaling {
+    int32_t kind;
+    int32_t original_max_pos; /* BANDS, YARN: > 0 */
+    double base;              /* > 0; YARN: > 1 */
+    double factor;            /* > 0 (not NONE) */
+    double low_freq_factor;   /* BANDS: 0 < low < high */
+    double high_freq_factor;
+    double beta_fast;         /* YARN: > 0 each */
+    double beta_slow;
+    double attention_factor;  /* 0: the kind's own; else > 0 */
+} af_rope_scaling;
+
+/* Host-only, in 64 bits: the rot_dim / 2 angles per position and the factor on cos
+ * and sin. rot_dim up to 256. */
+int af_rope_frequencies(const af_rope_scaling* scaling, int rot_dim, double* h_freq,
+                        double* h_factor);
+
+/* Rows [first_pos, first_pos + n_rows) of the table of positions, in one launch:
+ *   d_cos[r, i] = cos((first_pos + r) h_freq[i]) * factor, d_sin likewise,
+ * rows of rot_dim / 2 floats, the first at d_cos and d_sin (16-byte aligned).
+ * h_freq is host memory and read before the call returns (a captured launch keeps the
+ * values). Angles are reduced in 64 bits: each value is the exact one rounded to fp32
+ * (off by no more than 0.51 steps of it, or 2^-50 n where the angle's n turns cost more).
+ * The tables serve every entry point that takes cos_table and sin_table; those of the
+ * unscaled form are af_rope_table_build's within its fp32 arithmetic. */
+int af_rope_table_scaled(float* d_cos, float* d_sin, int64_t first_pos, int n_rows, int rot_dim,
+                         const double* h_freq, double factor, af_stream_t stream);
+
+/* Rotary positions of m rows: q_out[i] = row q[i] turned by table row d_positions[i] (p0 + i
+ * where d_positions is NULL), heads h at + h * head_dim, likewise k (k NULL or n_k_heads 0:
+ * q alone). Outputs may be the inputs themselves (same pointer and stride), else they
+ * overlap nothing. inverse = 1 turns back. Strides in elements, >= heads * head_dim;
+ * fp16 rows of any alignment (16 bytes, with rot_dim a multiple of 16, run fastest). Arithmetic as
+ * af_rope's: with AF_ROPE_HALF and rot_dim = head_dim the same bits. A row whose position is not
+ * in [0, max_pos) is left (copied) unturned, and AF_ERR_OUT_OF_RANGE stored into *d_status
+ * (if given). Tables: [max_pos, rot_dim / 2] fp32, 16-byte aligned. */
+int af_rope_rows(const void* q, int64_t q_stride, void* q_out, int64_t q_out_stride, int n_q_heads,
+                 const void* k, int64_t k_stride, void* k_out, int64_t k_out_stride, int n_k_heads,
+                 int m, int head_dim, int rot_dim, int layout, int inverse, const float* cos_table,
+                 const float* sin_table, int max_pos, const int32_t* d_positions, int p0,
+                 int32_t* d_status, af_stream_t stream);
+
+/* af_paged_rope_append in these forms: of m rows qkv[i] = [Q | K | V], Q turned into q_out, K
+ * turned and V as it is into row d_slots[i] of the pool's layer. qkv is only read (q_out may
+ * be qkv itself, with its stride: then the Q part is turned in place and K and V left). Slot
+ * -1: a row that is not cached (padding); another slot outside the pool, or a position outside
+ * [0, max_pos) (whose Q is copied unturned), caches nothing either and stores AF_ERR_OUT_OF_RANGE into
+ * *d_status (if given). The slots of one call are distinct. FP8 pools: K and V / scale,
+ * clamped to +-448 and rounded once, from the fp32 value (af_paged_rope_append rounds K to
+ * fp16 first); NaN stays NaN. */
+int af_paged_rope_append_rows(const void* qkv, int64_t qkv_stride, int m, void* q_out,
+                              int64_t q_out_stride, int n_q_heads, const af_kv_pool* pool,
+                              int layer, const int64_t* d_slots, const int32_t* d_positions,
+                              int rot_dim, int layout, const float* cos_table,
+                              const float* sin_table, int max_pos, int32_t* d_status,
+                              af_stream_t stream);
+
 /* Paged GQA decode attention for a batch.
  * q: [batch, q_stride] fp16 (head h at q + b*q_stride + h*head_dim),
  * d_block_tables: [batch, max_blocks_per_seq] int32, d_seq_lens: [batch] int32,
@@ -307,6 +394,30 @@ int af_paged_gather(const af_kv_pool* pool, int layer, const int32_t* d_block_ta
  * d_copies[3i+1], K and V, all layers. max_copies bounds *d_count. */
 int af_kv_copy_blocks(const af_kv_pool* pool, const int32_t* d_copies, const int32_t* d_count,
                       int max_copies, af_stream_t stream);
+
+/* Rows dropped out of cached sequences: what stays moves up, every layer, in one launch.
+ * For sequence s, with n = d_start[s + 1] - d_start[s] rows that move and f = d_first[s] rows
+ * before them that stay where they are:
+ *   logical row f + i  <-  logical row d_keep[d_start[s] + i],   i = 0 .. n - 1,
+ * through d_dst_tables[s] and d_src_tables[s] ([n_seqs][max_blocks] block ids each; the same
+ * tables for a sequence that moves in place, other blocks where its own are shared:
+ * af_bm_plan_compact makes both). d_keep is strictly increasing within a sequence, with
+ * d_keep[d_start[s] + i] >= f + i; then every row is read before it is written, whatever else
+ * moves. No destination block is another sequence's source or destination.
+ * rot_dim > 0: K is turned back by the rows' way up, from its position to its new one, in
+ * fp32 and rounded once (FP8: in units of its codes, clamped to +-448), with row
+ * d_keep[..] - (f + i) of the tables ([max_pos, rot_dim / 2]; a table that holds a
+ * factor other than 1 on cos and sin names it in table_factor). rot_dim 0: the rows keep
+ * their bits (rows that stand for themselves at any place; the tables may be NULL).
+ * A row whose source or destination lies past max_blocks * block_size, whose block id is outside
+ * the pool, that would move down, or whose way up is not in the tables is left out, and
+ * AF_ERR_OUT_OF_RANGE stored into *d_status (if given). max_rows: at least the longest
+ * sequence's n (rows past it are left out, silently); it sizes the launch. */
+int af_kv_compact(const af_kv_pool* pool, const int32_t* d_src_tables, const int32_t* d_dst_tables,
+                  int max_blocks, int n_seqs, const int32_t* d_keep, const int32_t* d_start,
+                  const int32_t* d_first, int max_rows, int rot_dim, int layout,
+                  const float* cos_table, const float* sin_table, int max_pos, float table_factor,
+                  int32_t* d_status, af_stream_t stream);
 
 /* FP8 E4M3 quantisation of fp16 values with one fp32 scale (device). */
 int af_fp8_quantize(const void* src_f16, uint8_t* dst, size_t n, float scale, af_stream_t stream);
@@ -438,6 +549,45 @@ int af_w8a8_gemm(const int8_t* x, int64_t x_stride, const float* x_scales, int m
  * own on (one row of tiles, more than 12 MB of weights). One token: 1 and the
  * weight rows of a wave, 1, 0, 1. Every form gives the same bits. m >= 1. */
 int af_w8a8_gemm_form(int m, int n, int k, int32_t* form);
+
+/* ======================================================================== */
+/* b1". Low-rank adapters beside a shared projection                         */
+/* ======================================================================== */
+/* The adapters of one projection, n_adapters slots of one layer:
+ *   a  fp16 [n_adapters][n_slices][max_rank][k],  b  fp16 [n_adapters][n][max_rank],
+ * 16-byte aligned. Slice s is the product's columns [slice_end[s-1], slice_end[s]) (a fused QKV or
+ * gate and up weight has one low-rank pair per part; slice_end[n_slices-1] = n).
+ * ranks: device int32 [n_adapters], an adapter's own rank (0 .. max_rank, clamped; NULL: max_rank for
+ * all): what a and b hold behind it is not used. scales: device fp32 [n_adapters] or NULL
+ * (1). max_rank: a multiple of 8, at most 128; k a multiple of 8. */
+#define AF_LORA_MAX_SLICES 4
+typedef struct af_lora {
+    const void* a;
+    const void* b;
+    const int32_t* ranks;
+    const float* scales;
+    int32_t n_adapters;
+    int32_t max_rank;
+    int32_t n_slices;
+    int32_t k;
+    int32_t n;
+    int32_t slice_end[AF_LORA_MAX_SLICES];
+} af_lora;
+
+/* Workspace bytes for launches of up to m tokens (0 on bad arguments). Needs no
+ * initialisation; launches that share one must be ordered. */
+size_t af_lora_workspace_size(const af_lora* lora, int m);
+/* Adds each token's adapter to a projection that the tokens share (af_w8a16_gemm_batched's,
+ * af_w8a8_gemm's; x is that projection's fp16 input):
+ *   y_out[i, j] = y[i, j] + scale * sum_r b[id, j, r] (sum_k a[id, s(j), r, k] x[i, k]),
+ * id = d_ids[i], r < rank of id, s(j) the slice of column j. A token whose id is outside [0, n_adapters)
+ * (-1: none), or whose adapter has rank 0, keeps y, bit for bit. Tokens of several adapters come in any order.
+ * x rows x_stride elements apart (a multiple of 8, x 16-byte aligned); y and y_out rows of y_dtype (AF_FP16 or
+ * AF_FP32), any alignment of their elements; y_out may be y (same stride), else they overlap nothing. fp32 sums, rounded once to
+ * y_dtype. A token's row has the same bits whatever m and the other tokens are. m up to 2^20. */
+int af_lora_add(const void* x, int64_t x_stride, int m, const int32_t* d_ids, const af_lora* lora,
+                const void* y, int64_t y_stride, void* y_out, int64_t y_out_stride, int y_dtype,
+                void* workspace, size_t workspace_bytes, af_stream_t stream);
 
 /* ======================================================================== */
 /* b2. Prefill: multi-token append and causal attention over a prompt chunk */
@@ -627,6 +777,21 @@ int af_bm_plan_decode(af_block_manager* bm, const int32_t* seqs, int n, int64_t*
  * bookkeeping: paged_kv_manager.h:51,61). hold: AF_OK or AF_ERR_BAD_BLOCK. */
 int af_bm_hold_copy_source(af_block_manager* bm, int block_id);
 int af_bm_release_copy_sources(af_block_manager* bm);
+/* Cuts n sequences (none twice) to some of their rows: sequence i keeps its logical rows
+ * keep[keep_start[i]] .. keep[keep_start[i + 1] - 1], strictly increasing and within its length, and
+ * is that many tokens long afterwards (none: empty). Writes what af_kv_compact then reads, to host
+ * arrays: src_tables and dst_tables [n][max_blocks] (unused entries 0), moved (the rows that move, at most
+ * as many as keep has), start [n + 1], first [n], *max_rows (0: nothing to launch). Rows in front of
+ * the first one dropped stay in place. A block that has other references, or is held as a copy's source,
+ * is left as it is and replaced by a new one. The moves are launched before anything that writes to blocks
+ * handed out later (a block freed here may be one of their sources), and after the copies that are planned
+ * already. Not for sequences that a scheduler runs. On an error (AF_ERR_POOL_EXHAUSTED, AF_ERR_BAD_SEQUENCE,
+ * AF_ERR_OUT_OF_RANGE: a row outside the sequence, or max_blocks below a sequence's blocks,
+ * AF_ERR_INVALID_ARG) nothing changes. */
+int af_bm_plan_compact(af_block_manager* bm, const int32_t* seqs, int n, const int32_t* keep,
+                       const int32_t* keep_start, int32_t* src_tables, int32_t* dst_tables,
+                       int max_blocks, int32_t* moved, int32_t* start, int32_t* first,
+                       int32_t* max_rows);
 /* Block tables [n][max_blocks] (unused entries = 0) and lengths for n sequences. */
 int af_bm_export_tables(const af_block_manager* bm, const int32_t* seqs, int n, int32_t* tables,
                         int max_blocks, int32_t* seq_lens);

@@ -63,6 +63,17 @@ struct AppendSlot {
     CowCopy cow;
 };
 
+// What af_kv_compact reads to carry out plan_compact (its arguments of these names).
+struct CompactPlan {
+    int max_blocks = 0;                  // columns of the tables
+    std::vector<int32_t> src_tables;     // [n][max_blocks]
+    std::vector<int32_t> dst_tables;
+    std::vector<int32_t> keep;           // rows that move, sequence after sequence
+    std::vector<int32_t> start;          // [n + 1]
+    std::vector<int32_t> first;          // [n]
+    int max_rows = 0;
+};
+
 struct PoolConfig {
     int total_blocks = 0;
     int block_size = BLOCK_SIZE;
@@ -119,6 +130,16 @@ public:
     int append_token(int seq, AppendSlot* out);
     int extend(int seq, int n_tokens, int* first_pos, CowCopy* cow);
     int plan_decode(const int* seqs, int n, AppendSlot* out);
+    // Cuts each of n sequences (no one twice) to its rows keep[keep_start[i]] ..
+    // keep[keep_start[i + 1] - 1] (logical rows, strictly increasing), in that order, and says
+    // how the rows move. Blocks that nobody else references are written in place; a block
+    // with other references (or held as a copy's source) keeps its rows, and the sequence gets a
+    // new one. AF_ERR_POOL_EXHAUSTED, _BAD_SEQUENCE, _OUT_OF_RANGE, _INVALID_ARG: nothing changed.
+    // Blocks that become free are handed out again by later calls, so the moves are launched
+    // before anything that writes to blocks planned later. Sequences that a Scheduler runs are not
+    // for this call: it counts their tokens and shared rows itself.
+    int plan_compact(const int* seqs, int n, const int* keep, const int* keep_start,
+                     CompactPlan* out);
 
 private:
     struct Undo {
