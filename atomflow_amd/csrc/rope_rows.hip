@@ -15,6 +15,7 @@ namespace {
 constexpr double kTwoPi = 6.283185307179586476925286766559;
 constexpr int kMaxPairs = 128;  // rot_dim up to 256
 constexpr int kMaxHeadDim = 512;
+constexpr int kTableBlocks = 2048;  // 8 to a compute unit
 
 // ---- the table -------------------------------------------------------------------------------
 struct TableArgs {
@@ -54,26 +55,27 @@ __device__ __forceinline__ void turned(double t, double& c, double& s) {
     if (quarter >= 2) s = -s;
 }
 
-// V pairs of one position per thread.
+// V neighbouring pairs per thread, of every `step`-th row: their turns stay in registers.
 template <int V>
 __global__ __launch_bounds__(256) void rope_table_kernel(const TableArgs p) {
-    __shared__ double turns[kMaxPairs];
-    // (the arguments lie in memory: an index into them that differs by lane would go through
-    // private memory, so the copy's index is a loop's)
-    for (int i = 0; i < p.pairs; ++i)
-        if (int(threadIdx.x) == i) turns[i] = p.turns[i];
-    __syncthreads();
-    const int chunks = p.pairs / V;
-    const int64_t total = int64_t(p.n_rows) * chunks;
-    for (int64_t w = int64_t(blockIdx.x) * 256 + threadIdx.x; w < total;
-         w += int64_t(gridDim.x) * 256) {
-        const int row = int(w / chunks), i0 = int(w % chunks) * V;
+    const int chunks = p.pairs / V, rows = 256 / chunks;
+    const int i0 = int(threadIdx.x) % chunks * V, lane_row = int(threadIdx.x) / chunks;
+    if (lane_row >= rows) return;
+    // (the arguments as memory: an index into a by-value argument that differs by lane would go
+    // through private memory)
+    typedef const __attribute__((address_space(4))) TableArgs* Args;
+    const Args args = (Args)__builtin_amdgcn_kernarg_segment_ptr();
+    double turns[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) turns[i] = args->turns[i0 + i];
+    const int64_t step = int64_t(gridDim.x) * rows;
+    for (int64_t row = int64_t(blockIdx.x) * rows + lane_row; row < p.n_rows; row += step) {
         const double pos = double(p.first + row);
         float c[V], s[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             double cd, sd;
-            turned(pos * turns[i0 + i], cd, sd);
+            turned(pos * turns[i], cd, sd);
             c[i] = float(cd * p.factor);
             s[i] = float(sd * p.factor);
         }
@@ -334,8 +336,7 @@ extern "C" int af_rope_table_scaled(float* d_cos, float* d_sin, int64_t first_po
     if (n_rows == 0) return AF_OK;
     if (!d_cos || !d_sin || !on(d_cos, 16) || !on(d_sin, 16)) return AF_ERR_INVALID_ARG;
     const int v = a.pairs % 4 == 0 ? 4 : 1;
-    const int64_t items = int64_t(n_rows) * (a.pairs / v);
-    const int grid = int(std::min<int64_t>((items + 255) / 256, 8192));
+    const int grid = std::min(ceil_div(n_rows, 256 / (a.pairs / v)), kTableBlocks);
     if (v == 4)
         hipLaunchKernelGGL(rope_table_kernel<4>, dim3(grid), dim3(256), 0,
                            static_cast<hipStream_t>(stream), a);
