@@ -3,20 +3,22 @@
 //   y_out[i, j] = y[i, j] + scale[a] * sum_r B[a, j, r] * v[i, s(j), r],   a = ids[i]
 //   v[i, s, r]  = sum_k A[a, s, r, k] x[i, k],                             r < rank[a]
 //
-// Two launches. `down` computes v: tiles of 16 or 64 tokens, K cut into at most eight parts whose
-// sums it leaves in the workspace. `up` adds the parts, and its tiles' products to y. Both run on
-// the matrix cores (16x16x32, fp16 operands, fp32 sums), with the adapter's rows as the first
-// operand and the tokens as the second, so a token's sums depend on no other token.
+// Two launches. `down` computes v over tiles of up to 64 tokens; K is cut into at most eight parts,
+// whose sums it leaves in the workspace, or adds itself where the tiles alone fill the device. `up`
+// adds the parts, and its tiles' products to y. Both run on the matrix cores (16x16x32, fp16
+// operands, fp32 sums), with the adapter's rows as the first operand and the tokens as the second,
+// so a token's sums depend on no other token.
 //
-// Tokens come in any order. A tile's workgroups (grid z) each take one of the adapters that its
-// tokens name, every J-th from z on, compute the whole tile with that adapter's weights and write
-// the rows that are its own: a prompt's tile has one adapter, a decode batch's tile of 16 has up
-// to 16, side by side. No plan, no sort, no host data: ids, ranks and scales may change between
-// the replays of a graph.
+// Tokens come in any order. A tile's workgroups (grid z) each take some of the adapters that its
+// tokens name, every J-th from z on, and gather that adapter's tokens, 16 to an operand: a prompt's
+// tile has one adapter, a decode batch's up to 64, side by side, and the weights of each are read once
+// per tile. No plan, no sort, no host data: ids, ranks and scales may change between the replays of a
+// graph.
 //
 // Sums: K's parts and the order in which they are added are fixed by k alone, and every form adds
 // a token's products in the same order, so a token's row has the same bits whatever the launch.
 #include <algorithm>
+#include <type_traits>
 
 #include "af_common.h"
 #include "af_device.h"
@@ -33,6 +35,10 @@ typedef float f32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
 
 constexpr int kMaxSlices = AF_LORA_MAX_SLICES;
 constexpr int kMaxRank = 128;
+constexpr int kTile = 64;     // tokens of a tile: one to a lane
+constexpr int kCols = 256;    // `up`: columns of a workgroup, the gathering form's
+constexpr int kSpan = 1024;   // and the other one's
+constexpr int kGroup = 8;     // `up`: column blocks that a tile's workgroups take one after the other
 constexpr int kParts = 8;     // parts of K, at most
 constexpr int kPartMin = 512; // k of a part, at least
 
@@ -50,12 +56,14 @@ struct LoraArgs {
     int64_t y_stride;
     void* y_out;
     int64_t y_out_stride;
-    float* v;               // [parts][m][rows]
+    float* v;               // [splits][m][rows]
     int parts, part_k;
+    int splits;             // parts, or 1: `down` adds them
+    int down_tile, tiles;   // tokens of a tile of `down`; `up`: tiles of kTile tokens
     int n_slices;
     int slice_begin[kMaxSlices + 1];
     int slice_block[kMaxSlices + 1];  // `up`: first column block of each slice
-    int cols;                         // `up`: columns of a workgroup
+    int items;                        // `up`: (column block, tile) pairs
 };
 
 __device__ __forceinline__ f16x8 load_f16x8(const uint16_t* p) {
@@ -66,103 +74,229 @@ __device__ __forceinline__ f16x8 load_f16x8(const uint16_t* p) {
 struct Adapters {
     uint64_t todo;
     int id;
+    uint64_t mask;  // the tokens of the adapter that next() found
+    int order;      // lane j: the j-th of them, counted in the tile
+    int count;      // how many
     __device__ __forceinline__ Adapters(int id, bool valid) : todo(__ballot(valid)), id(id) {}
-    // Skips `skip` adapters; false when there is none behind them. mask: the tokens of `adapter`.
-    __device__ __forceinline__ bool next(int skip, int& adapter, uint64_t& mask) {
+    // Skips `skip` adapters; false when there is none behind them.
+    __device__ __forceinline__ bool next(int skip, int& adapter) {
         while (todo) {
             const int lead = __builtin_ctzll(todo);
             adapter = __builtin_amdgcn_readlane(id, lead);
             mask = __ballot(id == adapter) & todo;
             todo &= ~mask;
-            if (skip-- == 0) return true;
+            if (skip-- > 0) continue;
+            // the adapter's tokens to the front lanes, the others behind them
+            const int lane = threadIdx.x & 63;
+            const uint64_t below = (uint64_t(1) << lane) - 1;
+            count = __builtin_popcountll(mask);
+            const int before = __builtin_popcountll(mask & below);
+            const int to = (mask >> lane) & 1 ? before : count + lane - before;
+            order = __builtin_amdgcn_ds_permute(4 * to, lane);
+            return true;
         }
         return false;
     }
+    // Token of place j (the last one where there are fewer).
+    __device__ __forceinline__ int token(int j) const { return __shfl(order, min(j, count - 1)); }
 };
 
+__device__ __forceinline__ int rank_of(const LoraArgs& p, int adapter) {
+    return p.ranks ? min(max(p.ranks[adapter], 0), p.rmax) : p.rmax;
+}
+
 // ---- down: v ------------------------------------------------------------------------------
-// MT 16-token tiles by NT 16-row tiles of A. The four waves take a quarter of the part's k each,
-// operands straight from memory into registers (no barrier in the loop); their sums meet in LDS.
+// A part of K is four chains of products, each from zero, added one after the other; then the parts
+// are. MT 16-token tiles by NT 16-row tiles of A in every wave, operands straight from memory into
+// registers.
 template <int MT, int NT>
-__global__ __launch_bounds__(256) void lora_down_kernel(const LoraArgs p) {
-    __shared__ f32x4 sums[4][MT * NT][64];
-    const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
-    const int t0 = blockIdx.x * (16 * MT);
-    const int part = blockIdx.y % p.parts;
-    const int row0 = (blockIdx.y / p.parts) * (16 * NT);
-    int id = -1;
-    if (lane < 16 * MT && t0 + lane < p.m) id = p.ids[t0 + lane];
-    Adapters todo(id, id >= 0 && id < p.n_adapters);
-
-    const int sub = 8 * (lane >> 4);
-    const uint16_t* xp[MT];
+struct Operands {
+    const uint16_t* x[MT];
+    const uint16_t* a[NT];
+    __device__ __forceinline__ Operands(const LoraArgs& p, const Adapters& some, int t0, int base, int adapter,
+                                        int rank, int row0, int lane) {
+        const int sub = 8 * (lane >> 4);
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-        const int row = min(t0 + 16 * i + (lane & 15), p.m - 1);
-        xp[i] = p.x + size_t(row) * p.x_stride + sub;
-    }
-    const int kw = p.part_k / 4;
-    const int k0 = part * p.part_k + wave * kw;
-    const int k1 = min(k0 + kw, p.k);
-
-    int adapter;
-    uint64_t mask;
-    for (int skip = blockIdx.z; todo.next(skip, adapter, mask); skip = int(gridDim.z) - 1) {
-        const int rank = p.ranks ? min(max(p.ranks[adapter], 0), p.rmax) : p.rmax;
-        const uint16_t* ap[NT];
+        for (int i = 0; i < MT; ++i)
+            x[i] = p.x + size_t(t0 + some.token(base + 16 * i + (lane & 15))) * p.x_stride + sub;
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
             const int r = row0 + 16 * i + (lane & 15);
             const bool ok = r < p.rows && r % p.rmax < rank;
             // (a row past the rank touches its own sums alone, and those are not used)
-            ap[i] = p.a + (size_t(adapter) * p.rows + (ok ? r : row0)) * p.k + sub;
+            a[i] = p.a + (size_t(adapter) * p.rows + (ok ? r : row0)) * p.k + sub;
         }
-        f32x4 acc[MT][NT] = {};
-        int k = k0;
-        for (; k + 32 <= k1; k += 32) {
-            f16x8 xf[MT], af[NT];
+    }
+};
+
+template <int MT, int NT, int U>
+__device__ __forceinline__ void multiply(const f16x8 (&xf)[U][MT], const f16x8 (&af)[U][NT], int u,
+                                         f32x4 (&acc)[MT][NT]) {
 #pragma unroll
-            for (int i = 0; i < MT; ++i) xf[i] = load_f16x8(xp[i] + k);
+    for (int i = 0; i < MT; ++i)
 #pragma unroll
-            for (int i = 0; i < NT; ++i) af[i] = load_f16x8(ap[i] + k);
+        for (int j = 0; j < NT; ++j)
+            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(af[u][j], xf[u][i], acc[i][j], 0, 0, 0);
+}
+
+// A tile's sum s to v. Lane: token lane & 15, rows 4 * (lane >> 4) ... of the tile.
+__device__ __forceinline__ void store_v(const LoraArgs& p, const Adapters& some, int split, int t0, int place, int r,
+                                        int rank, f32x4 s) {
+    const int token = some.token(place);
+    if (place < some.count && r < p.rows) {
 #pragma unroll
-            for (int i = 0; i < MT; ++i)
+        for (int e = 0; e < 4; ++e)
+            if ((r + e) % p.rmax >= rank) s[e] = 0.0f;
+        *reinterpret_cast<f32x4*>(p.v + (size_t(split) * p.m + t0 + token) * p.rows + r) = s;
+    }
+}
+
+// Few tiles: a workgroup takes one part, a wave one of its chains, kUnroll steps' loads before the first
+// product. The four sums meet in LDS.
+template <int MT, int NT>
+__global__ __launch_bounds__(256) void lora_down_kernel(const LoraArgs p) {
+    constexpr int kUnroll = 4;
+    __shared__ f32x4 sums[4][MT * NT][64];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
+    const int t0 = blockIdx.x * p.down_tile;
+    const int part = blockIdx.y % p.parts;
+    const int row0 = (blockIdx.y / p.parts) * (16 * NT);
+    int id = -1;
+    if (lane < p.down_tile && t0 + lane < p.m) id = p.ids[t0 + lane];
+    Adapters todo(id, id >= 0 && id < p.n_adapters);
+    const int sub = 8 * (lane >> 4), kw = p.part_k / 4;
+    const int k0 = part * p.part_k + wave * kw, k1 = min(k0 + kw, p.k);
+
+    int adapter;
+    for (int skip = blockIdx.z; todo.next(skip, adapter); skip = int(gridDim.z) - 1) {
+        const int rank = rank_of(p, adapter);
+        if (rank == 0) continue;
+#pragma unroll 1
+        for (int base = 0; base < todo.count; base += 16 * MT) {
+            const Operands<MT, NT> at(p, todo, t0, base, adapter, rank, row0, lane);
+            f32x4 acc[MT][NT] = {};
+            f16x8 xf[kUnroll][MT], af[kUnroll][NT];
+            int k = k0;
+            for (; k + 32 * kUnroll <= k1; k += 32 * kUnroll) {
 #pragma unroll
-                for (int j = 0; j < NT; ++j)
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(af[j], xf[i], acc[i][j], 0, 0, 0);
-        }
-        if (k < k1) {  // k is a multiple of 8: whole pieces of 8, or none
-            const bool in = k + sub < k1;
-            f16x8 xf[MT], af[NT];
+                for (int u = 0; u < kUnroll; ++u) {
 #pragma unroll
-            for (int i = 0; i < MT; ++i) xf[i] = in ? load_f16x8(xp[i] + k) : f16x8{};
+                    for (int i = 0; i < MT; ++i) xf[u][i] = load_f16x8(at.x[i] + k + 32 * u);
 #pragma unroll
-            for (int i = 0; i < NT; ++i) af[i] = in ? load_f16x8(ap[i] + k) : f16x8{};
+                    for (int i = 0; i < NT; ++i) af[u][i] = load_f16x8(at.a[i] + k + 32 * u);
+                }
 #pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-                for (int j = 0; j < NT; ++j)
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(af[j], xf[i], acc[i][j], 0, 0, 0);
-        }
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int j = 0; j < NT; ++j) sums[wave][i * NT + j][lane] = acc[i][j];
-        __syncthreads();
-        // lane: token lane & 15 of the tile, rows 4 * (lane >> 4) ...
-        for (int t = wave; t < MT * NT; t += 4) {
-            const int token = 16 * (t / NT) + (lane & 15);
-            const int r = row0 + 16 * (t % NT) + 4 * (lane >> 4);
-            if (((mask >> token) & 1) && r < p.rows) {
-                f32x4 s = (sums[0][t][lane] + sums[1][t][lane]) + (sums[2][t][lane] + sums[3][t][lane]);
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if ((r + e) % p.rmax >= rank) s[e] = 0.0f;
-                *reinterpret_cast<f32x4*>(p.v + (size_t(part) * p.m + t0 + token) * p.rows + r) = s;
+                for (int u = 0; u < kUnroll; ++u) multiply<MT, NT>(xf, af, u, acc);
             }
+            if (k < k1) {  // k is a multiple of 8: whole pieces of 8, or none
+#pragma unroll
+                for (int u = 0; u < kUnroll; ++u) {
+                    const bool in = k + 32 * u + sub < k1;
+                    if (k + 32 * u >= k1) break;
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) xf[u][i] = in ? load_f16x8(at.x[i] + k + 32 * u) : f16x8{};
+#pragma unroll
+                    for (int i = 0; i < NT; ++i) af[u][i] = in ? load_f16x8(at.a[i] + k + 32 * u) : f16x8{};
+                }
+#pragma unroll
+                for (int u = 0; u < kUnroll; ++u) {
+                    if (k + 32 * u >= k1) break;
+                    multiply<MT, NT>(xf, af, u, acc);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) sums[wave][i * NT + j][lane] = acc[i][j];
+            __syncthreads();
+            for (int t = wave; t < MT * NT; t += 4)
+                store_v(p, todo, part, t0, base + 16 * (t / NT) + (lane & 15),
+                        row0 + 16 * (t % NT) + 4 * (lane >> 4), rank,
+                        ((sums[0][t][lane] + sums[1][t][lane]) + sums[2][t][lane]) + sums[3][t][lane]);
+            __syncthreads();
         }
-        __syncthreads();
+    }
+}
+
+// Many tiles: a workgroup takes all of K, a wave one part, whose sum it keeps in LDS from chain to
+// chain; the parts meet there at the end. Two steps' loads are on their way while the two before are
+// multiplied.
+template <int MT, int NT>
+__global__ __launch_bounds__(64 * kParts) void lora_down_all_kernel(const LoraArgs p) {
+    __shared__ f32x4 sums[kParts][MT * NT][64];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
+    const int t0 = blockIdx.x * kTile;
+    const int row0 = blockIdx.y * (16 * NT);
+    int id = -1;
+    if (t0 + lane < p.m) id = p.ids[t0 + lane];
+    Adapters todo(id, id >= 0 && id < p.n_adapters);
+    const int sub = 8 * (lane >> 4), kw = p.part_k / 4;
+    const int k0 = wave * p.part_k, k1 = min(k0 + p.part_k, p.k);
+
+    int adapter;
+    for (int skip = blockIdx.z; todo.next(skip, adapter); skip = int(gridDim.z) - 1) {
+        const int rank = rank_of(p, adapter);
+        if (rank == 0) continue;
+#pragma unroll 1
+        for (int base = 0; base < todo.count; base += 16 * MT) {
+            const Operands<MT, NT> at(p, todo, t0, base, adapter, rank, row0, lane);
+            f32x4 acc[MT][NT] = {};
+#pragma unroll
+            for (int t = 0; t < MT * NT; ++t) sums[wave][t][lane] = acc[0][0];
+            // (past K the loads repeat what is there, and x counts as zero)
+            auto load = [&](f16x8(&xf)[2][MT], f16x8(&af)[2][NT], int k) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const int off = min(k + 32 * u, p.k - 8 - sub);
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) xf[u][i] = load_f16x8(at.x[i] + off);
+#pragma unroll
+                    for (int i = 0; i < NT; ++i) af[u][i] = load_f16x8(at.a[i] + off);
+                }
+            };
+            auto work = [&](f16x8(&xf)[2][MT], f16x8(&af)[2][NT], int k) {
+                if (k + 64 > p.k) {
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int i = 0; i < MT; ++i)
+                            if (k + 32 * u + sub >= p.k) xf[u][i] = f16x8{};
+                }
+                multiply<MT, NT>(xf, af, 0, acc);
+                multiply<MT, NT>(xf, af, 1, acc);
+                if ((k + 64 - k0) % kw == 0) {  // a chain ends
+#pragma unroll
+                    for (int i = 0; i < MT; ++i)
+#pragma unroll
+                        for (int j = 0; j < NT; ++j) {
+                            asm volatile("" ::: "memory");  // (one at a time: registers)
+                            sums[wave][i * NT + j][lane] += acc[i][j];
+                            acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                        }
+                }
+            };
+            if (k0 < k1) {
+                f16x8 x0[2][MT], a0[2][NT], x1[2][MT], a1[2][NT];
+                load(x0, a0, k0);
+#pragma unroll 1
+                for (int k = k0; k < k0 + p.part_k; k += 128) {
+                    load(x1, a1, k + 64);
+                    work(x0, a0, k);
+                    load(x0, a0, k + 128);
+                    work(x1, a1, k + 64);
+                }
+            }
+            __syncthreads();
+            for (int t = wave; t < MT * NT; t += kParts) {
+                f32x4 s = sums[0][t][lane];
+                for (int q = 1; q < p.parts; ++q) s += sums[q][t][lane];
+                store_v(p, todo, 0, t0, base + 16 * (t / NT) + (lane & 15), row0 + 16 * (t % NT) + 4 * (lane >> 4),
+                        rank, s);
+            }
+            __syncthreads();
+        }
     }
 }
 
@@ -177,196 +311,431 @@ __device__ __forceinline__ int scale_exponent(float top) {
 
 __device__ __forceinline__ float pow2f(int e) { return __builtin_ldexpf(1.0f, e); }
 
+// Eight neighbouring elements of y as they lie in memory; load_part and store_part: n of them, 1 .. 8.
 template <typename Y>
-__device__ __forceinline__ void load_y16(const Y* p, int n, float (&v)[16]);
+struct Run8;
 template <>
-__device__ __forceinline__ void load_y16(const uint16_t* p, int n, float (&v)[16]) {
-    if (n >= 16) {
+struct Run8<uint16_t> {
+    u32x4 w;
+    __device__ __forceinline__ void load(const uint16_t* p) { w = *reinterpret_cast<const u32x4_a2*>(p); }
+    __device__ __forceinline__ void store(uint16_t* p) const { *reinterpret_cast<u32x4_a2*>(p) = w; }
+    __device__ __forceinline__ void load_part(const uint16_t* p, int n) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const u32x4_a2 w = *reinterpret_cast<const u32x4_a2*>(p + 8 * h);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[8 * h + i] = h2f(uint16_t(w[i >> 1] >> (16 * (i & 1))));
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = i < n ? h2f(p[i]) : 0.0f;
+        for (int i = 0; i < 4; ++i)
+            w[i] = p[min(2 * i, n - 1)] | uint32_t(p[min(2 * i + 1, n - 1)]) << 16;
     }
-}
+    __device__ __forceinline__ void store_part(uint16_t* p, int n) const {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < n) p[i] = uint16_t(w[i >> 1] >> (16 * (i & 1)));
+    }
+    __device__ __forceinline__ float get(int i) const { return h2f(uint16_t(w[i >> 1] >> (16 * (i & 1)))); }
+    __device__ __forceinline__ void set(const float (&v)[8]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = uint32_t(f2h(v[2 * i])) | (uint32_t(f2h(v[2 * i + 1])) << 16);
+    }
+};
 template <>
-__device__ __forceinline__ void load_y16(const float* p, int n, float (&v)[16]) {
-    if (n >= 16) {
-#pragma unroll
-        for (int h = 0; h < 4; ++h) {
-            const f32x4_a4 w = *reinterpret_cast<const f32x4_a4*>(p + 4 * h);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[4 * h + i] = w[i];
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = i < n ? p[i] : 0.0f;
+struct Run8<float> {
+    f32x4 w[2];
+    __device__ __forceinline__ void load(const float* p) {
+        w[0] = *reinterpret_cast<const f32x4_a4*>(p);
+        w[1] = *reinterpret_cast<const f32x4_a4*>(p + 4);
     }
-}
-__device__ __forceinline__ void store_y16(uint16_t* p, int n, const float (&v)[16]) {
-    if (n >= 16) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            u32x4_a2 w;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                w[i] = uint32_t(f2h(v[8 * h + 2 * i])) | (uint32_t(f2h(v[8 * h + 2 * i + 1])) << 16);
-            *reinterpret_cast<u32x4_a2*>(p + 8 * h) = w;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-            if (i < n) p[i] = f2h(v[i]);
+    __device__ __forceinline__ void store(float* p) const {
+        *reinterpret_cast<f32x4_a4*>(p) = w[0];
+        *reinterpret_cast<f32x4_a4*>(p + 4) = w[1];
     }
+    __device__ __forceinline__ void load_part(const float* p, int n) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i >> 2][i & 3] = p[min(i, n - 1)];
+    }
+    __device__ __forceinline__ void store_part(float* p, int n) const {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < n) p[i] = w[i >> 2][i & 3];
+    }
+    __device__ __forceinline__ float get(int i) const { return w[i >> 2][i & 3]; }
+    __device__ __forceinline__ void set(const float (&v)[8]) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i >> 2][i & 3] = v[i];
+    }
+};
+
+// v's fp16 halves of a tile, in LDS: rows of 32 KS ranks and 16 bytes.
+template <int KS>
+struct Halves {
+    static constexpr int kLd = 32 * KS + 8;
+    static constexpr int kPer = 8 * KS;  // threads that work on a token's v, four ranks each
+    __attribute__((aligned(16))) uint16_t hi[kTile * kLd];
+    __attribute__((aligned(16))) uint16_t lo[kTile * kLd];
+    float back[kTile];
+    // Ranks r0 .. r0 + 3 of slice s of token t: the parts' sums, times the scale.
+    static __device__ __forceinline__ f32x4 load(const LoraArgs& p, int t, int s, int r0, float scale,
+                                                 bool split) {
+        const float* src = p.v + size_t(t) * p.rows + s * p.rmax + r0;
+        f32x4 v = *reinterpret_cast<const f32x4*>(src);
+        if (split) {
+            const size_t step = size_t(p.m) * p.rows;
+            f32x4 part[kParts];
+#pragma unroll
+            for (int q = 1; q < kParts; ++q)
+                part[q] = *reinterpret_cast<const f32x4*>(src + min(q, p.splits - 1) * step);
+#pragma unroll
+            for (int q = 1; q < kParts; ++q)
+                if (q < p.splits) v += part[q];
+        }
+        return v * scale;
+    }
+    // The kPer threads of a place bring its v, in neighbouring lanes.
+    __device__ __forceinline__ void put(int place, int r0, f32x4 v) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = max(top, __builtin_bit_cast(uint32_t, float(v[i])) & 0x7fffffffu);
+#pragma unroll
+        for (int o = 1; o < kPer; o *= 2) top = max(top, uint32_t(__shfl_xor(int(top), o)));
+        const int e = scale_exponent(__builtin_bit_cast(float, top));
+        const float down = pow2f(-e);
+        uint16_t h[4], l[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float w = v[i] * down;
+            h[i] = f2h(w);
+            l[i] = (h[i] & 0x7c00u) == 0x7c00u ? uint16_t(0) : f2h(w - h2f(h[i]));
+        }
+        auto two = [](const uint16_t(&x)[4], int i) { return uint32_t(x[i]) | (uint32_t(x[i + 1]) << 16); };
+        *reinterpret_cast<uint2*>(hi + place * kLd + r0) = make_uint2(two(h, 0), two(h, 2));
+        *reinterpret_cast<uint2*>(lo + place * kLd + r0) = make_uint2(two(l, 0), two(l, 2));
+        if (r0 == 0) back[place] = pow2f(e);
+    }
+};
+
+// 64 columns of an adapter's B as four first operands: row 4 g + i of the t-th (g, i the result's lane
+// group and element) is column 32 (t / 2) + 8 g + 4 (t % 2) + i, so that a lane ends up with two runs
+// of 8 columns of one token, and a token's four lanes with 64 (fp16) bytes in a row.
+template <int KS>
+struct Columns {
+    f16x8 f[4][KS];
+    // From column c on, those below col1 (the others repeat the last one).
+    __device__ __forceinline__ void load(const LoraArgs& p, int adapter, int c, int col1, int rank, int lane) {
+        const int from = min(c, col1 - 1);
+        const int last = (rank - 1) & ~7;  // (ranks of the adapter alone are read)
+        const uint16_t* at = p.b + (size_t(adapter) * p.n + from) * p.rmax;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const int r = lane & 15;
+            const int col = 32 * (t >> 1) + 8 * (r >> 2) + 4 * (t & 1) + (r & 3);
+            const int off = min(col, col1 - 1 - from) * p.rmax;
+#pragma unroll
+            for (int q = 0; q < KS; ++q)
+                f[t][q] = load_f16x8(at + off + min(32 * q + 8 * (lane >> 4), last));
+        }
+    }
+    // What lies behind the adapter's rank is not used.
+    __device__ __forceinline__ void cut(int rank, int lane) {
+#pragma unroll
+        for (int q = 0; q < KS; ++q) {
+            u32x4 keep;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int r = 32 * q + 8 * (lane >> 4) + 2 * i;
+                keep[i] = (r < rank ? 0xffffu : 0u) | (r + 1 < rank ? 0xffff0000u : 0u);
+            }
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+                f[t][q] = __builtin_bit_cast(f16x8, __builtin_bit_cast(u32x4, f[t][q]) & keep);
+        }
+    }
+    // acc = B (hi + lo) of 16 places.
+    __device__ __forceinline__ void product(const Halves<KS>& v, int place, int lane, f32x4 (&acc)[4]) const {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) acc[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int q = 0; q < KS; ++q) {
+            const f16x8 h = load_f16x8(v.hi + place * Halves<KS>::kLd + 32 * q + 8 * (lane >> 4));
+            const f16x8 l = load_f16x8(v.lo + place * Halves<KS>::kLd + 32 * q + 8 * (lane >> 4));
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                acc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[u][q], l, acc[u], 0, 0, 0);
+                acc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f[u][q], h, acc[u], 0, 0, 0);
+            }
+        }
+    }
+};
+
+// Run `half` of a lane's two: y += up * acc.
+template <typename Y>
+__device__ __forceinline__ void add_run(Run8<Y>& y, const f32x4 (&acc)[4], int half, float up) {
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = y.get(e) + up * acc[2 * half + (e >> 2)][e & 3];
+    y.set(v);
 }
-__device__ __forceinline__ void store_y16(float* p, int n, const float (&v)[16]) {
-    if (n >= 16) {
+
+// Where a workgroup of `up` works: workgroups go round the eight XCDs, and each XCD gets neighbouring
+// items, which are the tiles by kGroup column blocks (whose part of B stays in its L2), then the next
+// column blocks.
+struct Place {
+    bool any;
+    int s, t0, col0, col1;
+    __device__ __forceinline__ Place(const LoraArgs& p, int tile, int cols) {
+        const int item = int(blockIdx.x % 8) * int(gridDim.x / 8) + int(blockIdx.x / 8);
+        any = item < p.items;
+        const int group = item / (p.tiles * kGroup), in_group = item - group * (p.tiles * kGroup);
+        const int width = max(1, min(kGroup, p.slice_block[p.n_slices] - group * kGroup));
+        const int block = group * kGroup + in_group % width;
+        t0 = in_group / width * tile;
+        s = 0;
+        while (s + 1 < p.n_slices && block >= p.slice_block[s + 1]) ++s;
+        col0 = p.slice_begin[s] + (block - p.slice_block[s]) * cols;
+        col1 = min(col0 + cols, p.slice_begin[s + 1]);
+    }
+};
+
+// A tile's rows as they are (no adapter, or one of rank 0): columns [col0, col1) of its gathered tokens.
+template <typename Y>
+__device__ __forceinline__ void copy_rows(const LoraArgs& p, const Adapters& some, int t0, int col0, int col1) {
+    const int runs = (col1 - col0 + 7) / 8, total = some.count * runs;
+#pragma unroll 1
+    for (int from = threadIdx.x; from - int(threadIdx.x) < total; from += 4 * 256) {
+        Run8<Y> r[4];
+        const Y* src[4];
+        Y* dst[4];
+        int n[4];
 #pragma unroll
-        for (int h = 0; h < 4; ++h)
-            *reinterpret_cast<f32x4_a4*>(p + 4 * h) =
-                f32x4_a4{v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]};
-    } else {
+        for (int u = 0; u < 4; ++u) {
+            const int i = min(from + 256 * u, total - 1);
+            const int t = t0 + some.token(i / runs), col = col0 + 8 * (i % runs);
+            n[u] = col1 - col;
+            src[u] = static_cast<const Y*>(p.y) + size_t(t) * p.y_stride + col;
+            dst[u] = static_cast<Y*>(p.y_out) + size_t(t) * p.y_out_stride + col;
+        }
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-            if (i < n) p[i] = v[i];
+        for (int u = 0; u < 4; ++u) {
+            if (n[u] >= 8)
+                r[u].load(src[u]);
+            else
+                r[u].load_part(src[u], n[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            if (from + 256 * u >= total) continue;
+            if (n[u] >= 8)
+                r[u].store(dst[u]);
+            else
+                r[u].store_part(dst[u], n[u]);
+        }
     }
 }
 
-// 16 * MT tokens by p.cols columns of one slice; rank up to 32 * KS. A wave takes 64 columns at a
-// time: four first operands whose rows are the columns 16 g + 4 t + i (g, i the result's lane
-// group and element, t the operand), so that a lane ends up with 16 columns in a row of one token.
+// A slice's last columns [c, col1), fewer than 64, of an adapter's gathered tokens.
+template <int KS, typename Y>
+__device__ __forceinline__ void last_columns(const LoraArgs& p, const Adapters& some, const Columns<KS>& b,
+                                             const Halves<KS>& halves, int t0, int c, int col1, int lane) {
+    const int sub = c + 8 * (lane >> 4), n = col1 - sub;
+#pragma unroll 1
+    for (int base = 0; base < some.count; base += 16) {
+        const int place = base + (lane & 15);
+        const size_t t = size_t(t0 + some.token(place));
+        f32x4 acc[4];
+        b.product(halves, place, lane, acc);
+        const float up = halves.back[place];
+        const Y* from = static_cast<const Y*>(p.y) + t * p.y_stride + sub;
+        Y* to = static_cast<Y*>(p.y_out) + t * p.y_out_stride + sub;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if (place >= some.count || n <= 32 * h) continue;
+            Run8<Y> z;
+            z.load_part(from + 32 * h, n - 32 * h);
+            add_run(z, acc, h, up);
+            z.store_part(to + 32 * h, n - 32 * h);
+        }
+    }
+}
+
+// Many tiles: a tile's tokens of one adapter, gathered, by kSpan columns of one slice; rank up to
+// 32 KS. v is read and cut in halves once; then each wave takes 64 columns at a time, whose B and y
+// have been on their way since the 64 columns before.
 template <int MT, int KS, typename Y>
-__global__ __launch_bounds__(256) void lora_up_kernel(const LoraArgs p) {
-    constexpr int kTokens = 16 * MT, kLd = 32 * KS + 8;
-    __shared__ __attribute__((aligned(16))) uint16_t hi[kTokens * kLd];
-    __shared__ __attribute__((aligned(16))) uint16_t lo[kTokens * kLd];
-    __shared__ float back[kTokens];
-    const int lane = threadIdx.x & 63;
+__global__ __launch_bounds__(256, 2) void lora_up_span_kernel(const LoraArgs p) {
+    constexpr int kPer = Halves<KS>::kPer, kSlots = 256 / kPer;
+    __shared__ Halves<KS> halves;
+    int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
-    const int t0 = blockIdx.y * kTokens;
-    int s = 0;
-    while (s + 1 < p.n_slices && int(blockIdx.x) >= p.slice_block[s + 1]) ++s;
-    const int col0 = p.slice_begin[s] + (int(blockIdx.x) - p.slice_block[s]) * p.cols;
-    const int col1 = min(col0 + p.cols, p.slice_begin[s + 1]);
+    const Place at(p, kTile, kSpan);
+    if (!at.any) return;
+    const bool copy = p.y != p.y_out;  // tokens without an adapter are copied
+    int id = -1;
+    const bool token_in = at.t0 + lane < p.m;
+    if (token_in) id = p.ids[at.t0 + lane];
+    if (id < 0 || id >= p.n_adapters) id = -1;
+    Adapters todo(id, token_in && (copy || id >= 0));
+    const int first = at.col0 + 64 * wave;
+    const int end = at.col0 + (at.col1 - at.col0) / 64 * 64;  // of the whole runs of 64 columns
+
+    int adapter;
+    for (int skip = blockIdx.z; todo.next(skip, adapter); skip = int(gridDim.z) - 1) {
+        asm volatile("" : "+v"(lane));  // (what hangs on the lane is not worked out, and kept, before)
+        const int rank = adapter >= 0 ? rank_of(p, adapter) : 0;
+        if (rank == 0) {  // y as it is, bit for bit
+            if (copy) copy_rows<Y>(p, todo, at.t0, at.col0, at.col1);
+            continue;
+        }
+        const float scale = p.scales ? p.scales[adapter] : 1.0f;
+        const int r0 = lane % kPer * 4;
+#pragma unroll 1
+        for (int base = 0; base < todo.count; base += kSlots) {
+            const int place = base + (64 * wave + lane) / kPer;
+            const int t = at.t0 + todo.token(place);
+            f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (place < todo.count && r0 < rank) v = Halves<KS>::load(p, t, at.s, r0, scale, p.splits > 1);
+            halves.put(place, r0, v);
+        }
+        __syncthreads();
+        for (int base = 0; base < todo.count; base += 16 * MT) {
+            if (first >= end) break;
+            const Y* from[MT];
+            Y* to[MT];
+            bool mine[MT];
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                const int place = base + 16 * i + (lane & 15);
+                const size_t t = size_t(at.t0 + todo.token(place));
+                from[i] = static_cast<const Y*>(p.y) + t * p.y_stride + 8 * (lane >> 4);
+                to[i] = static_cast<Y*>(p.y_out) + t * p.y_out_stride + 8 * (lane >> 4);
+                mine[i] = place < todo.count;
+            }
+            auto load_y = [&](Run8<Y>(&y)[MT][2], int c) {
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    y[i][0].load(from[i] + c);
+                    y[i][1].load(from[i] + c + 32);
+                }
+            };
+            auto work = [&](Run8<Y>(&y)[MT][2], Columns<KS>& b, int c) {
+                b.cut(rank, lane);
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    const int place = base + 16 * i + (lane & 15);
+                    f32x4 acc[4];
+                    b.product(halves, place, lane, acc);
+                    const float up = halves.back[place];
+                    add_run(y[i][0], acc, 0, up);
+                    add_run(y[i][1], acc, 1, up);
+                    if (mine[i]) {
+                        y[i][0].store(to[i] + c);
+                        y[i][1].store(to[i] + c + 32);
+                    }
+                }
+            };
+            // Two sets of registers in turn. The loads ahead are not conditional (past the end they
+            // repeat the last columns): a branch would make the compiler copy, and so await, them.
+            Columns<KS> b0, b1;
+            Run8<Y> y0[MT][2], y1[MT][2];
+            const int last = first + (end - 1 - first) / 256 * 256;
+            b0.load(p, adapter, first, at.col1, rank, lane);
+            load_y(y0, first);
+            int c = first;
+#pragma unroll 1
+            for (; c + 256 < end; c += 512) {
+                b1.load(p, adapter, c + 256, at.col1, rank, lane);
+                load_y(y1, c + 256);
+                work(y0, b0, c);
+                b0.load(p, adapter, min(c + 512, last), at.col1, rank, lane);
+                load_y(y0, min(c + 512, last));
+                work(y1, b1, c + 256);
+            }
+            if (c < end) work(y0, b0, c);
+        }
+        if (end < at.col1 && wave == (end - at.col0) / 64 % 4) {
+            Columns<KS> b;
+            b.load(p, adapter, end, at.col1, rank, lane);
+            b.cut(rank, lane);
+            last_columns<KS, Y>(p, todo, b, halves, at.t0, end, at.col1, lane);
+        }
+        __syncthreads();
+    }
+}
+
+// Fewer tiles: a tile's tokens of one adapter, gathered, by 256 columns of one slice, 64 to a wave. B
+// and y of the first 16 MT tokens are on their way while v is read and cut in halves.
+template <int MT, int KS, typename Y>
+__global__ __launch_bounds__(256, KS == 1 ? 4 : KS == 2 ? 3 : 2) void lora_up_kernel(const LoraArgs p) {
+    constexpr int kPer = Halves<KS>::kPer, kSlots = 256 / kPer;  // tokens whose v is read at a time
+    __shared__ Halves<KS> halves;
+    int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
+    const Place at(p, kTile, kCols);
+    if (!at.any) return;
+    const int c = at.col0 + 64 * wave;     // the wave's columns,
+    const bool whole = c + 64 <= at.col1;  // all of which there are
 
     const bool copy = p.y != p.y_out;  // tokens without an adapter are copied
     int id = -1;
-    const bool token_in = lane < kTokens && t0 + lane < p.m;
-    if (token_in) id = p.ids[t0 + lane];
+    const bool token_in = at.t0 + lane < p.m;
+    if (token_in) id = p.ids[at.t0 + lane];
     if (id < 0 || id >= p.n_adapters) id = -1;
     Adapters todo(id, token_in && (copy || id >= 0));
 
     int adapter;
-    uint64_t mask;
-    for (int skip = blockIdx.z; todo.next(skip, adapter, mask); skip = int(gridDim.z) - 1) {
-        int rank = 0;
-        if (adapter >= 0) rank = p.ranks ? min(max(p.ranks[adapter], 0), p.rmax) : p.rmax;
+    for (int skip = blockIdx.z; todo.next(skip, adapter); skip = int(gridDim.z) - 1) {
+        asm volatile("" : "+v"(lane));  // (what hangs on the lane is not worked out, and kept, before)
+        const int rank = adapter >= 0 ? rank_of(p, adapter) : 0;
         if (rank == 0) {  // y as it is, bit for bit
-            if (copy) {
-                const int cols = col1 - col0;
-                for (int t = 0; t < kTokens; ++t) {
-                    if (!((mask >> t) & 1)) continue;
-                    const Y* src = static_cast<const Y*>(p.y) + size_t(t0 + t) * p.y_stride + col0;
-                    Y* dst = static_cast<Y*>(p.y_out) + size_t(t0 + t) * p.y_out_stride + col0;
-                    for (int c = threadIdx.x; c < cols; c += 256) dst[c] = src[c];
-                }
-            }
+            if (copy) copy_rows<Y>(p, todo, at.t0, at.col0, at.col1);
             continue;
         }
-        {  // the parts' sums, times the scale, in two halves
-            constexpr int kPer = 256 / kTokens;      // threads of a token
-            constexpr int kEach = 32 * KS / kPer;    // ranks of a thread
-            const int t = threadIdx.x / kPer, r0 = (threadIdx.x % kPer) * kEach;
-            const float scale = p.scales ? p.scales[adapter] : 1.0f;
-            const bool mine = (mask >> t) & 1;
-            float v[kEach];
-#pragma unroll
-            for (int i = 0; i < kEach; ++i) v[i] = 0.0f;
-            if (mine) {
-                const float* src = p.v + size_t(t0 + t) * p.rows + s * p.rmax + r0;
-#pragma unroll
-                for (int i = 0; i < kEach; ++i) {
-                    if (r0 + i < rank) {
-                        float sum = src[i];
-                        for (int q = 1; q < p.parts; ++q) sum += src[size_t(q) * p.m * p.rows + i];
-                        v[i] = sum * scale;
-                    }
-                }
-            }
-            uint32_t top = 0;
-#pragma unroll
-            for (int i = 0; i < kEach; ++i)
-                top = max(top, __builtin_bit_cast(uint32_t, v[i]) & 0x7fffffffu);
-#pragma unroll
-            for (int o = 1; o < kPer; o *= 2) top = max(top, uint32_t(__shfl_xor(int(top), o)));
-            const int e = scale_exponent(__builtin_bit_cast(float, top));
-            const float down = pow2f(-e);
-#pragma unroll
-            for (int i = 0; i < kEach; ++i) {
-                const float w = v[i] * down;
-                const uint16_t h = f2h(w);
-                hi[t * kLd + r0 + i] = h;
-                lo[t * kLd + r0 + i] = (h & 0x7c00u) == 0x7c00u ? uint16_t(0) : f2h(w - h2f(h));
-            }
-            if (threadIdx.x % kPer == 0) back[t] = pow2f(e);
-        }
-        __syncthreads();
-        // which of a lane's 8 ranks there are: what lies behind an adapter's rank is not used
-        u32x4 keep[KS];
-#pragma unroll
-        for (int q = 0; q < KS; ++q)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int r = 32 * q + 8 * (lane >> 4) + 2 * i;
-                keep[q][i] = (r < rank ? 0xffffu : 0u) | (r + 1 < rank ? 0xffff0000u : 0u);
-            }
-        for (int c = col0 + 64 * wave; c < col1; c += 256) {
-            f16x8 bf[4][KS];
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                const int col = c + 16 * ((lane & 15) >> 2) + 4 * t + (lane & 3);
-                const uint16_t* bp =
-                    p.b + (size_t(adapter) * p.n + min(col, col1 - 1)) * p.rmax + 8 * (lane >> 4);
-#pragma unroll
-                for (int q = 0; q < KS; ++q) {
-                    u32x4 w = {0, 0, 0, 0};
-                    if (32 * q + 8 * (lane >> 4) < rank)
-                        w = *reinterpret_cast<const u32x4*>(bp + 32 * q) & keep[q];
-                    bf[t][q] = __builtin_bit_cast(f16x8, w);
-                }
-            }
-            const int col = c + 16 * (lane >> 4);
-            const int left = col1 - col;
+        Columns<KS> b;
+        b.load(p, adapter, c, at.col1, rank, lane);
+        // Tokens from place `base` on, 16 to a tile. (A place past the adapter's tokens reads the last
+        // one's y, and a wave without 64 columns reads anything that is there.)
+        auto row = [&](int place, int64_t stride) {
+            return size_t(at.t0 + todo.token(place)) * stride + c + 8 * (lane >> 4);
+        };
+        Run8<Y> y[MT][2];
+        auto load_y = [&](int base) {
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
-                if (((mask >> (16 * i)) & 0xffffu) == 0) continue;
-                const int t = 16 * i + (lane & 15);
-                const bool mine = ((mask >> t) & 1) && left > 0;
-                float y[16];
-                if (mine)
-                    load_y16(static_cast<const Y*>(p.y) + size_t(t0 + t) * p.y_stride + col, left, y);
-                f32x4 acc[4] = {};
+                const Y* run = static_cast<const Y*>(p.y) + row(base + 16 * i + (lane & 15), p.y_stride);
+                run = whole ? run : reinterpret_cast<const Y*>(p.v);
+                y[i][0].load(run);
+                y[i][1].load(run + 32);
+            }
+        };
+        load_y(0);
+        const float scale = p.scales ? p.scales[adapter] : 1.0f;
+        const int r0 = lane % kPer * 4;
+#pragma unroll 1
+        for (int base = 0; base < todo.count; base += kSlots) {
+            const int place = base + (64 * wave + lane) / kPer;
+            const int t = at.t0 + todo.token(place);
+            f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (place < todo.count && r0 < rank) v = Halves<KS>::load(p, t, at.s, r0, scale, p.splits > 1);
+            halves.put(place, r0, v);
+        }
+        __syncthreads();
+        b.cut(rank, lane);
+        if (whole) {
+#pragma unroll 1
+            for (int base = 0; base < todo.count; base += 16 * MT) {
+                if (base > 0) load_y(base);
 #pragma unroll
-                for (int q = 0; q < KS; ++q) {
-                    const f16x8 h = load_f16x8(hi + t * kLd + 32 * q + 8 * (lane >> 4));
-                    const f16x8 l = load_f16x8(lo + t * kLd + 32 * q + 8 * (lane >> 4));
-#pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        acc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(bf[u][q], l, acc[u], 0, 0, 0);
-                        acc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(bf[u][q], h, acc[u], 0, 0, 0);
+                for (int i = 0; i < MT; ++i) {
+                    const int place = base + 16 * i + (lane & 15);
+                    f32x4 acc[4];
+                    b.product(halves, place, lane, acc);
+                    const float up = halves.back[place];
+                    add_run(y[i][0], acc, 0, up);
+                    add_run(y[i][1], acc, 1, up);
+                    Y* run = static_cast<Y*>(p.y_out) + row(place, p.y_out_stride);
+                    if (place < todo.count) {
+                        y[i][0].store(run);
+                        y[i][1].store(run + 32);
                     }
                 }
-                if (mine) {
-                    const float up = back[t];
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) y[e] += up * acc[e >> 2][e & 3];
-                    store_y16(static_cast<Y*>(p.y_out) + size_t(t0 + t) * p.y_out_stride + col, left, y);
-                }
             }
+        } else if (c < at.col1) {  // the slice's last columns, fewer than 64
+            last_columns<KS, Y>(p, todo, b, halves, at.t0, c, at.col1, lane);
         }
         __syncthreads();
     }
@@ -392,14 +761,32 @@ int lora_check(const af_lora* l) {
     return begin == l->n ? AF_OK : AF_ERR_INVALID_ARG;
 }
 
-template <int MT>
 void launch_down(const LoraArgs& p, dim3 grid, int nt, hipStream_t s) {
     switch (nt) {
-        case 1: hipLaunchKernelGGL((lora_down_kernel<MT, 1>), grid, dim3(256), 0, s, p); break;
-        case 2: hipLaunchKernelGGL((lora_down_kernel<MT, 2>), grid, dim3(256), 0, s, p); break;
-        case 3: hipLaunchKernelGGL((lora_down_kernel<MT, 3>), grid, dim3(256), 0, s, p); break;
-        default: hipLaunchKernelGGL((lora_down_kernel<MT, 4>), grid, dim3(256), 0, s, p); break;
+        case 1: hipLaunchKernelGGL((lora_down_kernel<1, 1>), grid, dim3(256), 0, s, p); break;
+        case 2: hipLaunchKernelGGL((lora_down_kernel<1, 2>), grid, dim3(256), 0, s, p); break;
+        case 3: hipLaunchKernelGGL((lora_down_kernel<1, 3>), grid, dim3(256), 0, s, p); break;
+        default: hipLaunchKernelGGL((lora_down_kernel<1, 4>), grid, dim3(256), 0, s, p); break;
     }
+}
+void launch_down_all(const LoraArgs& p, dim3 grid, int nt, hipStream_t s) {
+    constexpr int kThreads = 64 * kParts;
+    switch (nt) {
+        case 1: hipLaunchKernelGGL((lora_down_all_kernel<4, 1>), grid, dim3(kThreads), 0, s, p); break;
+        case 2: hipLaunchKernelGGL((lora_down_all_kernel<4, 2>), grid, dim3(kThreads), 0, s, p); break;
+        case 3: hipLaunchKernelGGL((lora_down_all_kernel<4, 3>), grid, dim3(kThreads), 0, s, p); break;
+        default: hipLaunchKernelGGL((lora_down_all_kernel<4, 4>), grid, dim3(kThreads), 0, s, p); break;
+    }
+}
+
+template <int MT, typename Y>
+void launch_up_span(const LoraArgs& p, dim3 grid, hipStream_t s) {
+    if (p.rmax <= 32)
+        hipLaunchKernelGGL((lora_up_span_kernel<MT, 1, Y>), grid, dim3(256), 0, s, p);
+    else if (p.rmax <= 64)
+        hipLaunchKernelGGL((lora_up_span_kernel<MT, 2, Y>), grid, dim3(256), 0, s, p);
+    else
+        hipLaunchKernelGGL((lora_up_span_kernel<1, 4, Y>), grid, dim3(256), 0, s, p);
 }
 
 template <int MT, typename Y>
@@ -466,33 +853,54 @@ extern "C" int af_lora_add(const void* x, int64_t x_stride, int m, const int32_t
     p.y_out_stride = y_out_stride;
     p.v = static_cast<float*>(workspace);
     p.parts = parts_of(p.k);
-    p.part_k = int(align_up(size_t(ceil_div(p.k, p.parts)), 128));
+    p.part_k = int(align_up(size_t(ceil_div(p.k, p.parts)), 256));
     p.n_slices = lora->n_slices;
 
+    // the most adapters that n tokens in a row can name
+    auto named = [&](int n) { return std::min(std::min(m, n), p.n_adapters); };
     const int mt = m > 256 ? 4 : 1;
-    const int tiles = ceil_div(m, 16 * mt);
-    const int side = std::min(mt == 4 ? 4 : 16, p.n_adapters);
     hipStream_t s = static_cast<hipStream_t>(stream);
 
     const int row_tiles = ceil_div(p.rows, 16);
-    const int nt = std::min(4, row_tiles);
-    const dim3 down(tiles, p.parts * ceil_div(row_tiles, nt), side);
-    if (mt == 4)
-        launch_down<4>(p, down, nt, s);
-    else
-        launch_down<1>(p, down, nt, s);
+    const int nt = std::min(4, row_tiles), row_groups = ceil_div(row_tiles, nt);
+    p.tiles = ceil_div(m, kTile);
+    if (p.tiles * row_groups >= 192) {
+        p.splits = 1;
+        p.down_tile = kTile;
+        const dim3 grid(p.tiles, row_groups, std::min(named(kTile), std::max(2, 1024 / (p.tiles * row_groups))));
+        launch_down_all(p, grid, nt, s);
+    } else {
+        p.splits = p.parts;
+        p.down_tile = mt == 4 ? 16 : kTile;
+        const int tiles = ceil_div(m, p.down_tile);
+        const dim3 grid(tiles, p.parts * row_groups,
+                        std::min(named(p.down_tile), std::max(1, 4096 / (tiles * p.parts * row_groups))));
+        launch_down(p, grid, nt, s);
+    }
     AF_TRY_LAUNCH();
 
-    p.cols = mt == 4 ? 1024 : 256;
+    const bool span = mt == 4 && int64_t(m) * p.n >= int64_t(1024) * kTile * 512;
+    const int cols = span ? kSpan : kCols;
     int blocks = 0;
     for (int i = 0; i < p.n_slices; ++i) {
         p.slice_begin[i + 1] = lora->slice_end[i];
         p.slice_block[i] = blocks;
-        blocks += ceil_div(lora->slice_end[i] - p.slice_begin[i], p.cols);
+        blocks += ceil_div(lora->slice_end[i] - p.slice_begin[i], cols);
     }
     p.slice_block[p.n_slices] = blocks;
-    const dim3 up(blocks, tiles, std::min(mt == 4 ? 4 : 16, p.n_adapters + (y != y_out)));
-    if (up.y > 65535) return AF_ERR_UNSUPPORTED;
+    if (int64_t(blocks) * p.tiles > (1 << 22)) return AF_ERR_UNSUPPORTED;
+    p.items = blocks * p.tiles;
+    dim3 up(unsigned(align_up(size_t(p.items), 8)));
+    if (span) {
+        up.z = std::min(named(kTile) + (y != y_out), std::max(2, 2048 / p.items));
+        if (y_dtype == AF_FP16)
+            launch_up_span<4, uint16_t>(p, up, s);
+        else
+            launch_up_span<2, float>(p, up, s);
+        AF_TRY_LAUNCH();
+        return AF_OK;
+    }
+    up.z = std::min(named(kTile) + (y != y_out), std::max(1, 4096 / p.items));
     if (y_dtype == AF_FP16) {
         if (mt == 4)
             launch_up<4, uint16_t>(p, up, s);
@@ -500,7 +908,7 @@ extern "C" int af_lora_add(const void* x, int64_t x_stride, int m, const int32_t
             launch_up<1, uint16_t>(p, up, s);
     } else {
         if (mt == 4)
-            launch_up<4, float>(p, up, s);
+            launch_up<2, float>(p, up, s);
         else
             launch_up<1, float>(p, up, s);
     }

@@ -254,3 +254,32 @@ def test_lora_workspace_too_small(gpu):
         kv.launch_lora_add(c.dx.ptr, 64, 4, c.di, c.lora, c.dy.ptr, 8, c.do.ptr, 8, c.ws,
                            kv.lora_workspace_size(c.lora, 4) - 1)
     assert e.value.status == atomflow_amd.AF_ERR_WORKSPACE
+
+
+LARGE = [  # launches whose tiles fill the device: m, k, slice ends, max_rank, adapters
+    (12300, 72, [130], 8, 5), (12289, 520, [33], 24, 3), (12290, 1288, [20, 41], 24, 6),
+    (3100, 1304, [60, 120, 180, 215], 128, 3), (8300, 64, [2050, 4111], 16, 4), (4100, 64, [8200], 64, 3),
+    (2100, 64, [16400], 128, 5)]
+
+
+@pytest.mark.parametrize("m,k,ends,rmax,count", LARGE)
+@pytest.mark.parametrize("y_dtype,pad,off", [(np.float16, 3, 1), (np.float32, 0, 0)])
+def test_lora_large(gpu, m, k, ends, rmax, count, y_dtype, pad, off):
+    """Prompt chunks, runs of one token of each adapter, and tokens without one; in place too, and a
+    few of the rows alone, bit for bit."""
+    say(f"lora large m={m} k={k} ends={ends} rank={rmax} adapters={count} {np.dtype(y_dtype)}")
+    c = Case(m, k, ends, rmax, count, m + k, y_dtype=y_dtype)
+    at = np.arange(m)
+    c.ids[:] = np.where(at < 70, at % (count + 1) - 1, (at // 700) % (count + 1) - 1)
+    c.device(8 * pad, pad, off).call()
+    c.check()
+    got = c.do.get()
+    c.call(out=c.dy)
+    assert c.dy.get().tobytes() == got.tobytes()
+    some = np.concatenate([np.arange(60, 75), np.arange(m - 20, m)])
+    part = Case(len(some), k, ends, rmax, count, m + k, y_dtype=y_dtype)
+    for name in ("a", "b", "ranks", "scales"):
+        setattr(part, name, getattr(c, name))
+    part.x, part.y, part.ids = (t[some].copy() for t in (c.x, c.y, c.ids))
+    part.device().call()
+    assert part.do.get().tobytes() == got[some].tobytes()
