@@ -219,84 +219,126 @@ __global__ __launch_bounds__(256) void lora_down_kernel(const LoraArgs p) {
     }
 }
 
-// Many tiles: a workgroup takes all of K, a wave one part, whose sum it keeps in LDS from chain to
-// chain; the parts meet there at the end. Two steps' loads are on their way while the two before are
-// multiplied.
-template <int MT, int NT>
-__global__ __launch_bounds__(64 * kParts) void lora_down_all_kernel(const LoraArgs p) {
-    __shared__ f32x4 sums[kParts][MT * NT][64];
+// More tiles: 64 tokens by 16 NT rows, all waves on the same 64 of K at a time, which memory writes
+// straight to LDS (kStages pieces of 64 on their way), 8 lanes to the 128 bytes of a row. Neighbouring lanes
+// of a first or second operand are rows apart, so that loading operands from memory costs the address unit
+// 64 cycles an instruction; this way it is 16. A wave takes 16 of the tokens. With p.splits a workgroup takes
+// one part of K, else all of them.
+template <int NT>
+__global__ __launch_bounds__(256) void lora_down_lds_kernel(const LoraArgs p) {
+    constexpr int kRows = kTile + 16 * NT;       // LDS: the tokens' rows of x, then rows of A, of 128 bytes
+    constexpr int kStages = NT <= 2 ? 6 : 4;
+    constexpr int kLoadsA = (2 * NT + 3) / 4, kLoads = 2 + kLoadsA;  // of a wave, for each piece
+    __shared__ __attribute__((aligned(1024))) uint8_t stage[kStages][kRows * 128];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
     const int t0 = blockIdx.x * kTile;
-    const int row0 = blockIdx.y * (16 * NT);
+    const int split = blockIdx.y % p.splits;
+    const int row0 = (blockIdx.y / p.splits) * (16 * NT);
     int id = -1;
     if (t0 + lane < p.m) id = p.ids[t0 + lane];
     Adapters todo(id, id >= 0 && id < p.n_adapters);
-    const int sub = 8 * (lane >> 4), kw = p.part_k / 4;
-    const int k0 = wave * p.part_k, k1 = min(k0 + p.part_k, p.k);
+    const int k0 = p.splits == 1 ? 0 : split * p.part_k;
+    const int k1 = min(p.splits == 1 ? p.k : k0 + p.part_k, p.k);
+    const int pieces = (k1 - k0 + 63) / 64;  // (none: a part behind K)
+    const uint32_t lds0 = lds_address(stage);
 
     int adapter;
     for (int skip = blockIdx.z; todo.next(skip, adapter); skip = int(gridDim.z) - 1) {
         const int rank = rank_of(p, adapter);
         if (rank == 0) continue;
-#pragma unroll 1
-        for (int base = 0; base < todo.count; base += 16 * MT) {
-            const Operands<MT, NT> at(p, todo, t0, base, adapter, rank, row0, lane);
-            f32x4 acc[MT][NT] = {};
+        // Load j of a lane: row 8 j + lane / 8 of its 16 bytes; rows' 16 bytes are kept in the order
+        // (piece ^ row) & 7, so that an operand's lanes read different banks.
+        const int in_row = lane >> 3, piece = (lane & 7) ^ in_row;
+        // Rows that are not used stay as they are in LDS (they touch their own sums alone), but for one
+        // lane of each load, so that every load counts: lanes that ask for a line that others have asked
+        // for wait for it, one by one (a pass of 5 tokens with 59 copies took 60 us, without them 12).
+        const uint16_t* from[kLoads];
+        uint32_t to[kLoads];
+        bool on[kLoads];
 #pragma unroll
-            for (int t = 0; t < MT * NT; ++t) sums[wave][t][lane] = acc[0][0];
-            // (past K the loads repeat what is there, and x counts as zero)
-            auto load = [&](f16x8(&xf)[2][MT], f16x8(&af)[2][NT], int k) {
+        for (int j = 0; j < 2; ++j) {
+            const int r = 16 * wave + 8 * j + in_row;
+            from[j] = p.x + size_t(t0 + todo.token(r)) * p.x_stride;
+            to[j] = lds0 + uint32_t(16 * wave + 8 * j) * 128;
+            on[j] = r < todo.count || lane == 0;
+        }
+#pragma unroll
+        for (int j = 0; j < kLoadsA; ++j) {
+            const int first = 8 * ((wave + 4 * j) % (2 * NT));  // (two waves may load the same rows)
+            const int r = row0 + first + in_row;
+            const bool ok = r < p.rows && r % p.rmax < rank;
+            on[2 + j] = ok || lane == 0;
+            from[2 + j] = p.a + (size_t(adapter) * p.rows + (ok ? r : row0)) * p.k;
+            to[2 + j] = lds0 + uint32_t(kTile + first) * 128;
+        }
+        auto load = [&](int i) {
+            const int k = min(k0 + 64 * i + 8 * piece, p.k - 8);
+            const uint32_t at = uint32_t(i % kStages) * (kRows * 128);
+#pragma unroll
+            for (int j = 0; j < kLoads; ++j)
+                if (on[j]) lds_dma16(from[j] + k, to[j] + at);
+        };
+#pragma unroll
+        for (int i = 0; i < kStages - 1; ++i)
+            if (i < pieces) load(i);
+        const bool mine = 16 * wave < todo.count;
+        f32x4 acc[1][NT] = {}, part[NT] = {}, total[NT] = {};
+        const int kw = p.part_k / 4;
+        for (int i = 0; i < pieces; ++i) {
+            // piece i is there when at most the loads of those behind it are on their way
+            const int behind = min(kStages - 2, pieces - 1 - i);
+            if (behind >= 4)
+                wait_vmcnt<4 * kLoads>();
+            else if (behind == 3)
+                wait_vmcnt<3 * kLoads>();
+            else if (behind == 2)
+                wait_vmcnt<2 * kLoads>();
+            else if (behind == 1)
+                wait_vmcnt<kLoads>();
+            else
+                wait_vmcnt<0>();
+            __syncthreads();  // (and every wave is done with piece i - 1, whose place the next load takes)
+            if (i + kStages - 1 < pieces) load(i + kStages - 1);
+            if (mine) {
+                const uint8_t* at = stage[i % kStages];
+                f16x8 xf[2][1], af[2][NT];
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    const int off = min(k + 32 * u, p.k - 8 - sub);
+                    const int slot = 16 * (((4 * u + (lane >> 4)) ^ lane) & 7);
+                    auto get = [&](int row) {
+                        return __builtin_bit_cast(f16x8, *reinterpret_cast<const u32x4*>(at + (row + (lane & 15)) * 128 + slot));
+                    };
+                    xf[u][0] = get(16 * wave);
 #pragma unroll
-                    for (int i = 0; i < MT; ++i) xf[u][i] = load_f16x8(at.x[i] + off);
-#pragma unroll
-                    for (int i = 0; i < NT; ++i) af[u][i] = load_f16x8(at.a[i] + off);
+                    for (int j = 0; j < NT; ++j) af[u][j] = get(kTile + 16 * j);
                 }
-            };
-            auto work = [&](f16x8(&xf)[2][MT], f16x8(&af)[2][NT], int k) {
+                const int k = k0 + 64 * i;
                 if (k + 64 > p.k) {
 #pragma unroll
                     for (int u = 0; u < 2; ++u)
+                        if (k + 32 * u + 8 * (lane >> 4) >= p.k) {
+                            xf[u][0] = f16x8{};
 #pragma unroll
-                        for (int i = 0; i < MT; ++i)
-                            if (k + 32 * u + sub >= p.k) xf[u][i] = f16x8{};
-                }
-                multiply<MT, NT>(xf, af, 0, acc);
-                multiply<MT, NT>(xf, af, 1, acc);
-                if ((k + 64 - k0) % kw == 0) {  // a chain ends
-#pragma unroll
-                    for (int i = 0; i < MT; ++i)
-#pragma unroll
-                        for (int j = 0; j < NT; ++j) {
-                            asm volatile("" ::: "memory");  // (one at a time: registers)
-                            sums[wave][i * NT + j][lane] += acc[i][j];
-                            acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                            for (int j = 0; j < NT; ++j) af[u][j] = f16x8{};
                         }
                 }
-            };
-            if (k0 < k1) {
-                f16x8 x0[2][MT], a0[2][NT], x1[2][MT], a1[2][NT];
-                load(x0, a0, k0);
-#pragma unroll 1
-                for (int k = k0; k < k0 + p.part_k; k += 128) {
-                    load(x1, a1, k + 64);
-                    work(x0, a0, k);
-                    load(x0, a0, k + 128);
-                    work(x1, a1, k + 64);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) multiply<1, NT>(xf, af, u, acc);
+                const int done = k + 64 - k0;
+                if (done % kw == 0 || i + 1 == pieces) {  // a chain ends
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) part[j] += acc[0][j], acc[0][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                    if (done % p.part_k == 0 || i + 1 == pieces)  // and a part
+#pragma unroll
+                        for (int j = 0; j < NT; ++j) total[j] += part[j], part[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
                 }
             }
-            __syncthreads();
-            for (int t = wave; t < MT * NT; t += kParts) {
-                f32x4 s = sums[0][t][lane];
-                for (int q = 1; q < p.parts; ++q) s += sums[q][t][lane];
-                store_v(p, todo, 0, t0, base + 16 * (t / NT) + (lane & 15), row0 + 16 * (t % NT) + 4 * (lane >> 4),
-                        rank, s);
-            }
-            __syncthreads();
         }
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+            store_v(p, todo, split, t0, 16 * wave + (lane & 15), row0 + 16 * j + 4 * (lane >> 4), rank, total[j]);
+        __syncthreads();
     }
 }
 
@@ -463,13 +505,18 @@ struct Columns {
     }
 };
 
-// Run `half` of a lane's two: y += up * acc.
+// y += up * sum
 template <typename Y>
-__device__ __forceinline__ void add_run(Run8<Y>& y, const f32x4 (&acc)[4], int half, float up) {
+__device__ __forceinline__ void add_run(Run8<Y>& y, const f32x4 (&sum)[2], float up) {
     float v[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = y.get(e) + up * acc[2 * half + (e >> 2)][e & 3];
+    for (int e = 0; e < 8; ++e) v[e] = y.get(e) + up * sum[e >> 2][e & 3];
     y.set(v);
+}
+template <typename Y>
+__device__ __forceinline__ void add_run(Run8<Y>& y, const f32x4 (&acc)[4], int half, float up) {
+    const f32x4 sum[2] = {acc[2 * half], acc[2 * half + 1]};
+    add_run(y, sum, up);
 }
 
 // Where a workgroup of `up` works: workgroups go round the eight XCDs, and each XCD gets neighbouring
@@ -555,11 +602,16 @@ __device__ __forceinline__ void last_columns(const LoraArgs& p, const Adapters& 
 
 // Many tiles: a tile's tokens of one adapter, gathered, by kSpan columns of one slice; rank up to
 // 32 KS. v is read and cut in halves once; then each wave takes 64 columns at a time, whose B and y
-// have been on their way since the 64 columns before.
+// have been on their way since the 64 columns before. The products go through LDS, 16 tokens at a time, to
+// lanes that have y as it lies in memory: 8 lanes to the 64 columns of a token. (With a token's y in the
+// lanes that hold its products, neighbouring lanes are rows apart, and the address unit takes 64 cycles for
+// an instruction instead of 16.)
 template <int MT, int KS, typename Y>
 __global__ __launch_bounds__(256, 2) void lora_up_span_kernel(const LoraArgs p) {
     constexpr int kPer = Halves<KS>::kPer, kSlots = 256 / kPer;
+    constexpr int kTurnLd = 68;  // (16 rows of 16 bytes fall on different banks)
     __shared__ Halves<KS> halves;
+    __shared__ __attribute__((aligned(16))) float turned[4][16 * kTurnLd];
     int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
     const Place at(p, kTile, kSpan);
@@ -594,44 +646,46 @@ __global__ __launch_bounds__(256, 2) void lora_up_span_kernel(const LoraArgs p) 
         __syncthreads();
         for (int base = 0; base < todo.count; base += 16 * MT) {
             if (first >= end) break;
-            const Y* from[MT];
-            Y* to[MT];
-            bool mine[MT];
+            // run j of a lane: token 8 j + lane / 8, columns 8 (lane % 8) ...
+            const Y* from[2 * MT];
+            Y* to[2 * MT];
 #pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                const int place = base + 16 * i + (lane & 15);
-                const size_t t = size_t(at.t0 + todo.token(place));
-                from[i] = static_cast<const Y*>(p.y) + t * p.y_stride + 8 * (lane >> 4);
-                to[i] = static_cast<Y*>(p.y_out) + t * p.y_out_stride + 8 * (lane >> 4);
-                mine[i] = place < todo.count;
+            for (int j = 0; j < 2 * MT; ++j) {
+                const size_t t = size_t(at.t0 + todo.token(base + 8 * j + (lane >> 3)));
+                from[j] = static_cast<const Y*>(p.y) + t * p.y_stride + 8 * (lane & 7);
+                to[j] = static_cast<Y*>(p.y_out) + t * p.y_out_stride + 8 * (lane & 7);
             }
-            auto load_y = [&](Run8<Y>(&y)[MT][2], int c) {
+            auto load_y = [&](Run8<Y>(&y)[2 * MT], int c) {
 #pragma unroll
-                for (int i = 0; i < MT; ++i) {
-                    y[i][0].load(from[i] + c);
-                    y[i][1].load(from[i] + c + 32);
-                }
+                for (int j = 0; j < 2 * MT; ++j) y[j].load(from[j] + c);
             };
-            auto work = [&](Run8<Y>(&y)[MT][2], Columns<KS>& b, int c) {
+            auto work = [&](Run8<Y>(&y)[2 * MT], Columns<KS>& b, int c) {
                 b.cut(rank, lane);
 #pragma unroll
                 for (int i = 0; i < MT; ++i) {
-                    const int place = base + 16 * i + (lane & 15);
                     f32x4 acc[4];
-                    b.product(halves, place, lane, acc);
-                    const float up = halves.back[place];
-                    add_run(y[i][0], acc, 0, up);
-                    add_run(y[i][1], acc, 1, up);
-                    if (mine[i]) {
-                        y[i][0].store(to[i] + c);
-                        y[i][1].store(to[i] + c + 32);
+                    b.product(halves, base + 16 * i + (lane & 15), lane, acc);
+                    float* put = turned[wave] + (lane & 15) * kTurnLd + 8 * (lane >> 4);
+                    asm volatile("" ::: "memory");  // (the wave's own LDS operations keep their order)
+#pragma unroll
+                    for (int t = 0; t < 4; ++t)
+                        *reinterpret_cast<f32x4*>(put + 32 * (t >> 1) + 4 * (t & 1)) = acc[t];
+                    asm volatile("" ::: "memory");
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int j = 2 * i + h, place = base + 8 * j + (lane >> 3);
+                        const float* get = turned[wave] + (8 * h + (lane >> 3)) * kTurnLd + 8 * (lane & 7);
+                        const f32x4 sum[2] = {*reinterpret_cast<const f32x4*>(get),
+                                              *reinterpret_cast<const f32x4*>(get + 4)};
+                        add_run(y[j], sum, halves.back[place]);
+                        if (place < todo.count) y[j].store(to[j] + c);
                     }
                 }
             };
             // Two sets of registers in turn. The loads ahead are not conditional (past the end they
             // repeat the last columns): a branch would make the compiler copy, and so await, them.
             Columns<KS> b0, b1;
-            Run8<Y> y0[MT][2], y1[MT][2];
+            Run8<Y> y0[2 * MT], y1[2 * MT];
             const int last = first + (end - 1 - first) / 256 * 256;
             b0.load(p, adapter, first, at.col1, rank, lane);
             load_y(y0, first);
@@ -769,13 +823,12 @@ void launch_down(const LoraArgs& p, dim3 grid, int nt, hipStream_t s) {
         default: hipLaunchKernelGGL((lora_down_kernel<1, 4>), grid, dim3(256), 0, s, p); break;
     }
 }
-void launch_down_all(const LoraArgs& p, dim3 grid, int nt, hipStream_t s) {
-    constexpr int kThreads = 64 * kParts;
+void launch_down_lds(const LoraArgs& p, dim3 grid, int nt, hipStream_t s) {
     switch (nt) {
-        case 1: hipLaunchKernelGGL((lora_down_all_kernel<4, 1>), grid, dim3(kThreads), 0, s, p); break;
-        case 2: hipLaunchKernelGGL((lora_down_all_kernel<4, 2>), grid, dim3(kThreads), 0, s, p); break;
-        case 3: hipLaunchKernelGGL((lora_down_all_kernel<4, 3>), grid, dim3(kThreads), 0, s, p); break;
-        default: hipLaunchKernelGGL((lora_down_all_kernel<4, 4>), grid, dim3(kThreads), 0, s, p); break;
+        case 1: hipLaunchKernelGGL(lora_down_lds_kernel<1>, grid, dim3(256), 0, s, p); break;
+        case 2: hipLaunchKernelGGL(lora_down_lds_kernel<2>, grid, dim3(256), 0, s, p); break;
+        case 3: hipLaunchKernelGGL(lora_down_lds_kernel<3>, grid, dim3(256), 0, s, p); break;
+        default: hipLaunchKernelGGL(lora_down_lds_kernel<4>, grid, dim3(256), 0, s, p); break;
     }
 }
 
@@ -864,11 +917,10 @@ extern "C" int af_lora_add(const void* x, int64_t x_stride, int m, const int32_t
     const int row_tiles = ceil_div(p.rows, 16);
     const int nt = std::min(4, row_tiles), row_groups = ceil_div(row_tiles, nt);
     p.tiles = ceil_div(m, kTile);
-    if (p.tiles * row_groups >= 192) {
-        p.splits = 1;
-        p.down_tile = kTile;
-        const dim3 grid(p.tiles, row_groups, std::min(named(kTile), std::max(2, 1024 / (p.tiles * row_groups))));
-        launch_down_all(p, grid, nt, s);
+    if (mt == 4 && p.tiles * row_groups * p.parts >= 192) {
+        p.splits = p.tiles * row_groups >= 192 ? 1 : p.parts;
+        const int groups = p.tiles * row_groups * p.splits;
+        launch_down_lds(p, dim3(p.tiles, row_groups * p.splits, std::min(named(kTile), std::max(2, 1024 / groups))), nt, s);
     } else {
         p.splits = p.parts;
         p.down_tile = mt == 4 ? 16 : kTile;
@@ -879,7 +931,7 @@ extern "C" int af_lora_add(const void* x, int64_t x_stride, int m, const int32_t
     }
     AF_TRY_LAUNCH();
 
-    const bool span = mt == 4 && int64_t(m) * p.n >= int64_t(1024) * kTile * 512;
+    const bool span = mt == 4 && int64_t(p.tiles) * p.n >= int64_t(1024) * kSpan;
     const int cols = span ? kSpan : kCols;
     int blocks = 0;
     for (int i = 0; i < p.n_slices; ++i) {
