@@ -9,8 +9,8 @@
 // operands, fp32 sums), with the adapter's rows as the first operand and the tokens as the second,
 // so a token's sums depend on no other token.
 //
-// Tokens come in any order. A tile's workgroups (grid z) each take some of the adapters that its
-// tokens name, every J-th from z on, and gather that adapter's tokens, 16 to an operand: a prompt's
+// Tokens come in any order. A tile's workgroups each take some of the adapters that its tokens
+// name, every J-th from the j-th on, and gather that adapter's tokens, 16 to an operand: a prompt's
 // tile has one adapter, a decode batch's up to 64, side by side, and the weights of each are read once
 // per tile. No plan, no sort, no host data: ids, ranks and scales may change between the replays of a
 // graph.
@@ -59,7 +59,8 @@ struct LoraArgs {
     float* v;               // [splits][m][rows]
     int parts, part_k;
     int splits;             // parts, or 1: `down` adds them
-    int down_tile, tiles;   // tokens of a tile of `down`; `up`: tiles of kTile tokens
+    int down_tile, down_tiles, down_items, down_side;  // `down`: tokens of a tile, tiles, (tile, rows, part)s
+    int tiles, side;        // `up`: tiles of kTile tokens
     int n_slices;
     int slice_begin[kMaxSlices + 1];
     int slice_block[kMaxSlices + 1];  // `up`: first column block of each slice
@@ -68,6 +69,15 @@ struct LoraArgs {
 
 __device__ __forceinline__ f16x8 load_f16x8(const uint16_t* p) {
     return __builtin_bit_cast(f16x8, *reinterpret_cast<const u32x4*>(p));
+}
+
+// Where `there` is false, any value: lanes that ask again for a line that is on its way wait for it one by
+// one, so what is not used is not loaded.
+__device__ __forceinline__ f16x8 load_f16x8_if(bool there, const uint16_t* p) {
+    f16x8 v;
+    v = __builtin_nondeterministic_value(v);
+    if (there) v = load_f16x8(p);
+    return v;
 }
 
 // The adapters that a tile's tokens name, in order of first appearance. Lane t holds token t's.
@@ -105,6 +115,22 @@ __device__ __forceinline__ int rank_of(const LoraArgs& p, int adapter) {
     return p.ranks ? min(max(p.ranks[adapter], 0), p.rmax) : p.rmax;
 }
 
+// Workgroups go round the eight XCDs. An item has `side` of them, which share out its tile's adapters: first
+// every item's first one, then every item's second one, most of which find nothing to do. (Workgroups
+// start in order, dealt out to an XCD's shader engines in turn, and one that finds no room there keeps those
+// behind it waiting. Side by side instead, two to an item, all first ones fell on half of the engines, at
+// twice the time; and the order is one further in each round, so that a tile of many adapters has its
+// workgroups on different engines.)
+struct Turn {
+    int xcd, nth, skip;  // nth item of the XCD
+    __device__ __forceinline__ explicit Turn(int items) {
+        const int per_xcd = (items + 7) / 8, i = int(blockIdx.x) / 8;
+        xcd = int(blockIdx.x) % 8;
+        skip = i / per_xcd;
+        nth = (i + skip) % per_xcd;
+    }
+};
+
 // ---- down: v ------------------------------------------------------------------------------
 // A part of K is four chains of products, each from zero, added one after the other; then the parts
 // are. MT 16-token tiles by NT 16-row tiles of A in every wave, operands straight from memory into
@@ -113,18 +139,21 @@ template <int MT, int NT>
 struct Operands {
     const uint16_t* x[MT];
     const uint16_t* a[NT];
+    bool x_on[MT], a_on[NT];  // (what a lane does not have touches its own sums alone, and those are not used)
     __device__ __forceinline__ Operands(const LoraArgs& p, const Adapters& some, int t0, int base, int adapter,
                                         int rank, int row0, int lane) {
         const int sub = 8 * (lane >> 4);
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
-            x[i] = p.x + size_t(t0 + some.token(base + 16 * i + (lane & 15))) * p.x_stride + sub;
+        for (int i = 0; i < MT; ++i) {
+            const int place = base + 16 * i + (lane & 15);
+            x[i] = p.x + size_t(t0 + some.token(place)) * p.x_stride + sub;
+            x_on[i] = place < some.count;
+        }
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
             const int r = row0 + 16 * i + (lane & 15);
-            const bool ok = r < p.rows && r % p.rmax < rank;
-            // (a row past the rank touches its own sums alone, and those are not used)
-            a[i] = p.a + (size_t(adapter) * p.rows + (ok ? r : row0)) * p.k + sub;
+            a_on[i] = r < p.rows && r % p.rmax < rank;
+            a[i] = p.a + (size_t(adapter) * p.rows + r) * p.k + sub;
         }
     }
 };
@@ -151,90 +180,108 @@ __device__ __forceinline__ void store_v(const LoraArgs& p, const Adapters& some,
     }
 }
 
-// Few tiles: a workgroup takes one part, a wave one of its chains, kUnroll steps' loads before the first
-// product. The four sums meet in LDS.
-template <int MT, int NT>
+// Up to 16 tokens of an adapter, from place `base` on, by all four waves: of each of the parts, a wave takes
+// one chain, kUnroll steps' loads before the first product; the four sums meet in LDS.
+template <int NT>
+__device__ __forceinline__ void few_tokens(const LoraArgs& p, const Adapters& todo, f32x4 (&sums)[4][NT][64], int t0,
+                                           int base, int adapter, int rank, int row0, int part0, int part1,
+                                           int split, int lane, int wave) {
+    constexpr int kUnroll = 4, kOwn = (NT + 3) / 4;
+    const Operands<1, NT> at(p, todo, t0, base, adapter, rank, row0, lane);
+    const int sub = 8 * (lane >> 4), kw = p.part_k / 4;
+    f32x4 total[kOwn] = {};
+#pragma unroll 1
+    for (int part = part0; part < part1; ++part) {
+        f32x4 acc[1][NT] = {};
+        f16x8 xf[kUnroll][1], af[kUnroll][NT];
+        int k = part * p.part_k + wave * kw;
+        const int k1 = min(k + kw, p.k);
+#pragma unroll 1
+        for (; k + 32 * kUnroll <= k1; k += 32 * kUnroll) {
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) {
+                xf[u][0] = load_f16x8_if(at.x_on[0], at.x[0] + k + 32 * u);
+#pragma unroll
+                for (int i = 0; i < NT; ++i) af[u][i] = load_f16x8_if(at.a_on[i], at.a[i] + k + 32 * u);
+            }
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) multiply<1, NT>(xf, af, u, acc);
+        }
+        if (k < k1) {  // k is a multiple of 8: whole pieces of 8, or none
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) {
+                const bool in = k + 32 * u + sub < k1;
+                if (k + 32 * u >= k1) break;
+                xf[u][0] = in && at.x_on[0] ? load_f16x8(at.x[0] + k + 32 * u) : f16x8{};
+#pragma unroll
+                for (int i = 0; i < NT; ++i) af[u][i] = in && at.a_on[i] ? load_f16x8(at.a[i] + k + 32 * u) : f16x8{};
+            }
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) {
+                if (k + 32 * u >= k1) break;
+                multiply<1, NT>(xf, af, u, acc);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < NT; ++j) sums[wave][j][lane] = acc[0][j];
+        __syncthreads();
+#pragma unroll
+        for (int o = 0; o < kOwn; ++o) {
+            const int t = min(wave + 4 * o, NT - 1);
+            total[o] += ((sums[0][t][lane] + sums[1][t][lane]) + sums[2][t][lane]) + sums[3][t][lane];
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int o = 0; o < kOwn; ++o) {
+        const int t = wave + 4 * o;
+        if (t >= NT) break;
+        store_v(p, todo, split, t0, base + (lane & 15), row0 + 16 * t + 4 * (lane >> 4), rank, total[o]);
+    }
+}
+
+// Few tiles: a workgroup takes one part.
+template <int NT>
 __global__ __launch_bounds__(256) void lora_down_kernel(const LoraArgs p) {
-    constexpr int kUnroll = 4;
-    __shared__ f32x4 sums[4][MT * NT][64];
+    __shared__ f32x4 sums[4][NT][64];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
-    const int t0 = blockIdx.x * p.down_tile;
-    const int part = blockIdx.y % p.parts;
-    const int row0 = (blockIdx.y / p.parts) * (16 * NT);
+    const Turn turn(p.down_items);
+    const int item = 8 * turn.nth + turn.xcd;
+    if (item >= p.down_items) return;
+    const int t0 = item % p.down_tiles * p.down_tile, rest = item / p.down_tiles;
+    const int part = rest % p.parts, row0 = rest / p.parts * (16 * NT);
     int id = -1;
     if (lane < p.down_tile && t0 + lane < p.m) id = p.ids[t0 + lane];
     Adapters todo(id, id >= 0 && id < p.n_adapters);
-    const int sub = 8 * (lane >> 4), kw = p.part_k / 4;
-    const int k0 = part * p.part_k + wave * kw, k1 = min(k0 + kw, p.k);
-
     int adapter;
-    for (int skip = blockIdx.z; todo.next(skip, adapter); skip = int(gridDim.z) - 1) {
+    for (int skip = turn.skip; todo.next(skip, adapter); skip = p.down_side - 1) {
         const int rank = rank_of(p, adapter);
         if (rank == 0) continue;
 #pragma unroll 1
-        for (int base = 0; base < todo.count; base += 16 * MT) {
-            const Operands<MT, NT> at(p, todo, t0, base, adapter, rank, row0, lane);
-            f32x4 acc[MT][NT] = {};
-            f16x8 xf[kUnroll][MT], af[kUnroll][NT];
-            int k = k0;
-            for (; k + 32 * kUnroll <= k1; k += 32 * kUnroll) {
-#pragma unroll
-                for (int u = 0; u < kUnroll; ++u) {
-#pragma unroll
-                    for (int i = 0; i < MT; ++i) xf[u][i] = load_f16x8(at.x[i] + k + 32 * u);
-#pragma unroll
-                    for (int i = 0; i < NT; ++i) af[u][i] = load_f16x8(at.a[i] + k + 32 * u);
-                }
-#pragma unroll
-                for (int u = 0; u < kUnroll; ++u) multiply<MT, NT>(xf, af, u, acc);
-            }
-            if (k < k1) {  // k is a multiple of 8: whole pieces of 8, or none
-#pragma unroll
-                for (int u = 0; u < kUnroll; ++u) {
-                    const bool in = k + 32 * u + sub < k1;
-                    if (k + 32 * u >= k1) break;
-#pragma unroll
-                    for (int i = 0; i < MT; ++i) xf[u][i] = in ? load_f16x8(at.x[i] + k + 32 * u) : f16x8{};
-#pragma unroll
-                    for (int i = 0; i < NT; ++i) af[u][i] = in ? load_f16x8(at.a[i] + k + 32 * u) : f16x8{};
-                }
-#pragma unroll
-                for (int u = 0; u < kUnroll; ++u) {
-                    if (k + 32 * u >= k1) break;
-                    multiply<MT, NT>(xf, af, u, acc);
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-                for (int j = 0; j < NT; ++j) sums[wave][i * NT + j][lane] = acc[i][j];
-            __syncthreads();
-            for (int t = wave; t < MT * NT; t += 4)
-                store_v(p, todo, part, t0, base + 16 * (t / NT) + (lane & 15),
-                        row0 + 16 * (t % NT) + 4 * (lane >> 4), rank,
-                        ((sums[0][t][lane] + sums[1][t][lane]) + sums[2][t][lane]) + sums[3][t][lane]);
-            __syncthreads();
-        }
+        for (int base = 0; base < todo.count; base += 16)
+            few_tokens<NT>(p, todo, sums, t0, base, adapter, rank, row0, part, part + 1, part, lane, wave);
     }
 }
 
 // More tiles: 64 tokens by 16 NT rows, all waves on the same 64 of K at a time, which memory writes
-// straight to LDS (kStages pieces of 64 on their way), 8 lanes to the 128 bytes of a row. Neighbouring lanes
+// straight to LDS (two pieces of 64 ahead), 8 lanes to the 128 bytes of a row. Neighbouring lanes
 // of a first or second operand are rows apart, so that loading operands from memory costs the address unit
 // 64 cycles an instruction; this way it is 16. A wave takes 16 of the tokens. With p.splits a workgroup takes
 // one part of K, else all of them.
 template <int NT>
 __global__ __launch_bounds__(256) void lora_down_lds_kernel(const LoraArgs p) {
     constexpr int kRows = kTile + 16 * NT;       // LDS: the tokens' rows of x, then rows of A, of 128 bytes
-    constexpr int kStages = NT <= 2 ? 6 : 4;
+    constexpr int kStages = 3;  // (with 6, two workgroups to a compute unit instead of three: 20 us became 30)
     constexpr int kLoadsA = (2 * NT + 3) / 4, kLoads = 2 + kLoadsA;  // of a wave, for each piece
     __shared__ __attribute__((aligned(1024))) uint8_t stage[kStages][kRows * 128];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
-    const int t0 = blockIdx.x * kTile;
-    const int split = blockIdx.y % p.splits;
-    const int row0 = (blockIdx.y / p.splits) * (16 * NT);
+    const Turn turn(p.down_items);
+    const int item = 8 * turn.nth + turn.xcd;
+    if (item >= p.down_items) return;
+    const int t0 = item % p.down_tiles * kTile, rest = item / p.down_tiles;
+    const int split = rest % p.splits, row0 = rest / p.splits * (16 * NT);
     int id = -1;
     if (t0 + lane < p.m) id = p.ids[t0 + lane];
     Adapters todo(id, id >= 0 && id < p.n_adapters);
@@ -244,9 +291,15 @@ __global__ __launch_bounds__(256) void lora_down_lds_kernel(const LoraArgs p) {
     const uint32_t lds0 = lds_address(stage);
 
     int adapter;
-    for (int skip = blockIdx.z; todo.next(skip, adapter); skip = int(gridDim.z) - 1) {
+    for (int skip = turn.skip; todo.next(skip, adapter); skip = p.down_side - 1) {
         const int rank = rank_of(p, adapter);
         if (rank == 0) continue;
+        if (todo.count <= 16) {
+            const int part = p.splits == 1 ? 0 : split;
+            few_tokens<NT>(p, todo, *reinterpret_cast<f32x4(*)[4][NT][64]>(stage), t0, 0, adapter, rank, row0, part,
+                           p.splits == 1 ? p.parts : part + 1, split, lane, wave);
+            continue;
+        }
         // Load j of a lane: row 8 j + lane / 8 of its 16 bytes; rows' 16 bytes are kept in the order
         // (piece ^ row) & 7, so that an operand's lanes read different banks.
         const int in_row = lane >> 3, piece = (lane & 7) ^ in_row;
@@ -259,7 +312,7 @@ __global__ __launch_bounds__(256) void lora_down_lds_kernel(const LoraArgs p) {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const int r = 16 * wave + 8 * j + in_row;
-            from[j] = p.x + size_t(t0 + todo.token(r)) * p.x_stride;
+            from[j] = p.x + size_t(t0 + todo.token(r)) * p.x_stride + k0 + 8 * piece;
             to[j] = lds0 + uint32_t(16 * wave + 8 * j) * 128;
             on[j] = r < todo.count || lane == 0;
         }
@@ -269,55 +322,57 @@ __global__ __launch_bounds__(256) void lora_down_lds_kernel(const LoraArgs p) {
             const int r = row0 + first + in_row;
             const bool ok = r < p.rows && r % p.rmax < rank;
             on[2 + j] = ok || lane == 0;
-            from[2 + j] = p.a + (size_t(adapter) * p.rows + (ok ? r : row0)) * p.k;
+            from[2 + j] = p.a + (size_t(adapter) * p.rows + (ok ? r : row0)) * p.k + k0 + 8 * piece;
             to[2 + j] = lds0 + uint32_t(kTile + first) * 128;
         }
-        auto load = [&](int i) {
-            const int k = min(k0 + 64 * i + 8 * piece, p.k - 8);
-            const uint32_t at = uint32_t(i % kStages) * (kRows * 128);
+        constexpr uint32_t kBytes = kRows * 128;
+        uint32_t fill = 0;  // the next load's place
+        int ahead = pieces;  // loads to come
+        auto load = [&] {
+            if (ahead == 0) return;
+            // (past K the loads repeat what is there)
+            int back = 0;
+            if (--ahead == 0) back = min(p.k - 8 - (k0 + 64 * (pieces - 1) + 8 * piece), 0);
 #pragma unroll
-            for (int j = 0; j < kLoads; ++j)
-                if (on[j]) lds_dma16(from[j] + k, to[j] + at);
+            for (int j = 0; j < kLoads; ++j) {
+                if (on[j]) lds_dma16(from[j] + back, to[j] + fill);
+                from[j] += 64;
+            }
+            fill = fill == (kStages - 1) * kBytes ? 0 : fill + kBytes;
         };
-#pragma unroll
-        for (int i = 0; i < kStages - 1; ++i)
-            if (i < pieces) load(i);
+        for (int i = 0; i < kStages - 1; ++i) load();
         const bool mine = 16 * wave < todo.count;
+        const int chain = p.part_k / 256;  // pieces of a chain
+        int in_chain = chain, chains = 4;  // left
+        uint32_t take = 0;
         f32x4 acc[1][NT] = {}, part[NT] = {}, total[NT] = {};
-        const int kw = p.part_k / 4;
-        for (int i = 0; i < pieces; ++i) {
-            // piece i is there when at most the loads of those behind it are on their way
-            const int behind = min(kStages - 2, pieces - 1 - i);
-            if (behind >= 4)
-                wait_vmcnt<4 * kLoads>();
-            else if (behind == 3)
-                wait_vmcnt<3 * kLoads>();
-            else if (behind == 2)
-                wait_vmcnt<2 * kLoads>();
-            else if (behind == 1)
+#pragma unroll 1
+        for (int left = pieces; left > 0; --left) {
+            // the piece is there when at most the loads of the next one are on their way
+            if (left > 1)
                 wait_vmcnt<kLoads>();
             else
                 wait_vmcnt<0>();
-            __syncthreads();  // (and every wave is done with piece i - 1, whose place the next load takes)
-            if (i + kStages - 1 < pieces) load(i + kStages - 1);
+            __syncthreads();  // (and every wave is done with the piece before, whose place the next load takes)
+            load();
             if (mine) {
-                const uint8_t* at = stage[i % kStages];
+                const uint8_t* at = stage[0] + take + (lane & 15) * 128;
                 f16x8 xf[2][1], af[2][NT];
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                     const int slot = 16 * (((4 * u + (lane >> 4)) ^ lane) & 7);
                     auto get = [&](int row) {
-                        return __builtin_bit_cast(f16x8, *reinterpret_cast<const u32x4*>(at + (row + (lane & 15)) * 128 + slot));
+                        return __builtin_bit_cast(f16x8, *reinterpret_cast<const u32x4*>(at + slot + row * 128));
                     };
                     xf[u][0] = get(16 * wave);
 #pragma unroll
                     for (int j = 0; j < NT; ++j) af[u][j] = get(kTile + 16 * j);
                 }
-                const int k = k0 + 64 * i;
-                if (k + 64 > p.k) {
+                if (left == 1) {
+                    const int k = k0 + 64 * (pieces - 1) + 8 * (lane >> 4);
 #pragma unroll
                     for (int u = 0; u < 2; ++u)
-                        if (k + 32 * u + 8 * (lane >> 4) >= p.k) {
+                        if (k + 32 * u >= p.k) {
                             xf[u][0] = f16x8{};
 #pragma unroll
                             for (int j = 0; j < NT; ++j) af[u][j] = f16x8{};
@@ -325,15 +380,18 @@ __global__ __launch_bounds__(256) void lora_down_lds_kernel(const LoraArgs p) {
                 }
 #pragma unroll
                 for (int u = 0; u < 2; ++u) multiply<1, NT>(xf, af, u, acc);
-                const int done = k + 64 - k0;
-                if (done % kw == 0 || i + 1 == pieces) {  // a chain ends
+                if (--in_chain == 0 || left == 1) {
 #pragma unroll
                     for (int j = 0; j < NT; ++j) part[j] += acc[0][j], acc[0][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-                    if (done % p.part_k == 0 || i + 1 == pieces)  // and a part
+                    in_chain = chain;
+                    if (--chains == 0 || left == 1) {
 #pragma unroll
                         for (int j = 0; j < NT; ++j) total[j] += part[j], part[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                        chains = 4;
+                    }
                 }
             }
+            take = take == (kStages - 1) * kBytes ? 0 : take + kBytes;
         }
 #pragma unroll
         for (int j = 0; j < NT; ++j)
@@ -359,6 +417,10 @@ struct Run8;
 template <>
 struct Run8<uint16_t> {
     u32x4 w;
+    __device__ __forceinline__ void load_if(bool there, const uint16_t* p) {
+        w = __builtin_nondeterministic_value(w);
+        if (there) load(p);
+    }
     __device__ __forceinline__ void load(const uint16_t* p) { w = *reinterpret_cast<const u32x4_a2*>(p); }
     __device__ __forceinline__ void store(uint16_t* p) const { *reinterpret_cast<u32x4_a2*>(p) = w; }
     __device__ __forceinline__ void load_part(const uint16_t* p, int n) {
@@ -380,6 +442,10 @@ struct Run8<uint16_t> {
 template <>
 struct Run8<float> {
     f32x4 w[2];
+    __device__ __forceinline__ void load_if(bool there, const float* p) {
+        w[0] = w[1] = __builtin_nondeterministic_value(w[0]);
+        if (there) load(p);
+    }
     __device__ __forceinline__ void load(const float* p) {
         w[0] = *reinterpret_cast<const f32x4_a4*>(p);
         w[1] = *reinterpret_cast<const f32x4_a4*>(p + 4);
@@ -461,7 +527,6 @@ struct Columns {
     // From column c on, those below col1 (the others repeat the last one).
     __device__ __forceinline__ void load(const LoraArgs& p, int adapter, int c, int col1, int rank, int lane) {
         const int from = min(c, col1 - 1);
-        const int last = (rank - 1) & ~7;  // (ranks of the adapter alone are read)
         const uint16_t* at = p.b + (size_t(adapter) * p.n + from) * p.rmax;
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
@@ -470,7 +535,7 @@ struct Columns {
             const int off = min(col, col1 - 1 - from) * p.rmax;
 #pragma unroll
             for (int q = 0; q < KS; ++q)
-                f[t][q] = load_f16x8(at + off + min(32 * q + 8 * (lane >> 4), last));
+                f[t][q] = load_f16x8_if(32 * q + 8 * (lane >> 4) < rank, at + off + 32 * q + 8 * (lane >> 4));
         }
     }
     // What lies behind the adapter's rank is not used.
@@ -519,14 +584,13 @@ __device__ __forceinline__ void add_run(Run8<Y>& y, const f32x4 (&acc)[4], int h
     add_run(y, sum, up);
 }
 
-// Where a workgroup of `up` works: workgroups go round the eight XCDs, and each XCD gets neighbouring
-// items, which are the tiles by kGroup column blocks (whose part of B stays in its L2), then the next
+// Where a workgroup of `up` works: each XCD gets neighbouring items, which are the tiles by kGroup column blocks (whose part of B stays in its L2), then the next
 // column blocks.
 struct Place {
     bool any;
     int s, t0, col0, col1;
-    __device__ __forceinline__ Place(const LoraArgs& p, int tile, int cols) {
-        const int item = int(blockIdx.x % 8) * int(gridDim.x / 8) + int(blockIdx.x / 8);
+    __device__ __forceinline__ Place(const LoraArgs& p, const Turn& turn, int tile, int cols) {
+        const int item = turn.xcd * ((p.items + 7) / 8) + turn.nth;
         any = item < p.items;
         const int group = item / (p.tiles * kGroup), in_group = item - group * (p.tiles * kGroup);
         const int width = max(1, min(kGroup, p.slice_block[p.n_slices] - group * kGroup));
@@ -614,7 +678,8 @@ __global__ __launch_bounds__(256, 2) void lora_up_span_kernel(const LoraArgs p) 
     __shared__ __attribute__((aligned(16))) float turned[4][16 * kTurnLd];
     int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
-    const Place at(p, kTile, kSpan);
+    const Turn turn(p.items);
+    const Place at(p, turn, kTile, kSpan);
     if (!at.any) return;
     const bool copy = p.y != p.y_out;  // tokens without an adapter are copied
     int id = -1;
@@ -626,7 +691,7 @@ __global__ __launch_bounds__(256, 2) void lora_up_span_kernel(const LoraArgs p) 
     const int end = at.col0 + (at.col1 - at.col0) / 64 * 64;  // of the whole runs of 64 columns
 
     int adapter;
-    for (int skip = blockIdx.z; todo.next(skip, adapter); skip = int(gridDim.z) - 1) {
+    for (int skip = turn.skip; todo.next(skip, adapter); skip = p.side - 1) {
         asm volatile("" : "+v"(lane));  // (what hangs on the lane is not worked out, and kept, before)
         const int rank = adapter >= 0 ? rank_of(p, adapter) : 0;
         if (rank == 0) {  // y as it is, bit for bit
@@ -657,7 +722,8 @@ __global__ __launch_bounds__(256, 2) void lora_up_span_kernel(const LoraArgs p) 
             }
             auto load_y = [&](Run8<Y>(&y)[2 * MT], int c) {
 #pragma unroll
-                for (int j = 0; j < 2 * MT; ++j) y[j].load(from[j] + c);
+                for (int j = 0; j < 2 * MT; ++j)
+                    y[j].load(from[j] + c);
             };
             auto work = [&](Run8<Y>(&y)[2 * MT], Columns<KS>& b, int c) {
                 b.cut(rank, lane);
@@ -719,7 +785,8 @@ __global__ __launch_bounds__(256, KS == 1 ? 4 : KS == 2 ? 3 : 2) void lora_up_ke
     __shared__ Halves<KS> halves;
     int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
-    const Place at(p, kTile, kCols);
+    const Turn turn(p.items);
+    const Place at(p, turn, kTile, kCols);
     if (!at.any) return;
     const int c = at.col0 + 64 * wave;     // the wave's columns,
     const bool whole = c + 64 <= at.col1;  // all of which there are
@@ -732,7 +799,7 @@ __global__ __launch_bounds__(256, KS == 1 ? 4 : KS == 2 ? 3 : 2) void lora_up_ke
     Adapters todo(id, token_in && (copy || id >= 0));
 
     int adapter;
-    for (int skip = blockIdx.z; todo.next(skip, adapter); skip = int(gridDim.z) - 1) {
+    for (int skip = turn.skip; todo.next(skip, adapter); skip = p.side - 1) {
         asm volatile("" : "+v"(lane));  // (what hangs on the lane is not worked out, and kept, before)
         const int rank = adapter >= 0 ? rank_of(p, adapter) : 0;
         if (rank == 0) {  // y as it is, bit for bit
@@ -741,8 +808,7 @@ __global__ __launch_bounds__(256, KS == 1 ? 4 : KS == 2 ? 3 : 2) void lora_up_ke
         }
         Columns<KS> b;
         b.load(p, adapter, c, at.col1, rank, lane);
-        // Tokens from place `base` on, 16 to a tile. (A place past the adapter's tokens reads the last
-        // one's y, and a wave without 64 columns reads anything that is there.)
+        // Tokens from place `base` on, 16 to a tile.
         auto row = [&](int place, int64_t stride) {
             return size_t(at.t0 + todo.token(place)) * stride + c + 8 * (lane >> 4);
         };
@@ -750,10 +816,11 @@ __global__ __launch_bounds__(256, KS == 1 ? 4 : KS == 2 ? 3 : 2) void lora_up_ke
         auto load_y = [&](int base) {
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
-                const Y* run = static_cast<const Y*>(p.y) + row(base + 16 * i + (lane & 15), p.y_stride);
-                run = whole ? run : reinterpret_cast<const Y*>(p.v);
-                y[i][0].load(run);
-                y[i][1].load(run + 32);
+                const int place = base + 16 * i + (lane & 15);
+                const Y* run = static_cast<const Y*>(p.y) + row(place, p.y_stride);
+                const bool there = whole && place < todo.count;
+                y[i][0].load_if(there, run);
+                y[i][1].load_if(there, run + 32);
             }
         };
         load_y(0);
@@ -817,10 +884,10 @@ int lora_check(const af_lora* l) {
 
 void launch_down(const LoraArgs& p, dim3 grid, int nt, hipStream_t s) {
     switch (nt) {
-        case 1: hipLaunchKernelGGL((lora_down_kernel<1, 1>), grid, dim3(256), 0, s, p); break;
-        case 2: hipLaunchKernelGGL((lora_down_kernel<1, 2>), grid, dim3(256), 0, s, p); break;
-        case 3: hipLaunchKernelGGL((lora_down_kernel<1, 3>), grid, dim3(256), 0, s, p); break;
-        default: hipLaunchKernelGGL((lora_down_kernel<1, 4>), grid, dim3(256), 0, s, p); break;
+        case 1: hipLaunchKernelGGL((lora_down_kernel<1>), grid, dim3(256), 0, s, p); break;
+        case 2: hipLaunchKernelGGL((lora_down_kernel<2>), grid, dim3(256), 0, s, p); break;
+        case 3: hipLaunchKernelGGL((lora_down_kernel<3>), grid, dim3(256), 0, s, p); break;
+        default: hipLaunchKernelGGL((lora_down_kernel<4>), grid, dim3(256), 0, s, p); break;
     }
 }
 void launch_down_lds(const LoraArgs& p, dim3 grid, int nt, hipStream_t s) {
@@ -917,17 +984,20 @@ extern "C" int af_lora_add(const void* x, int64_t x_stride, int m, const int32_t
     const int row_tiles = ceil_div(p.rows, 16);
     const int nt = std::min(4, row_tiles), row_groups = ceil_div(row_tiles, nt);
     p.tiles = ceil_div(m, kTile);
+    auto blocks_of = [](int items, int side) { return dim3(unsigned(align_up(size_t(items), 8)) * side); };
     if (mt == 4 && p.tiles * row_groups * p.parts >= 192) {
         p.splits = p.tiles * row_groups >= 192 ? 1 : p.parts;
-        const int groups = p.tiles * row_groups * p.splits;
-        launch_down_lds(p, dim3(p.tiles, row_groups * p.splits, std::min(named(kTile), std::max(2, 1024 / groups))), nt, s);
+        p.down_tiles = p.tiles;
+        p.down_items = p.tiles * row_groups * p.splits;
+        p.down_side = std::min(named(kTile), std::max(2, 1024 / p.down_items));
+        launch_down_lds(p, blocks_of(p.down_items, p.down_side), nt, s);
     } else {
         p.splits = p.parts;
         p.down_tile = mt == 4 ? 16 : kTile;
-        const int tiles = ceil_div(m, p.down_tile);
-        const dim3 grid(tiles, p.parts * row_groups,
-                        std::min(named(p.down_tile), std::max(1, 4096 / (tiles * p.parts * row_groups))));
-        launch_down(p, grid, nt, s);
+        p.down_tiles = ceil_div(m, p.down_tile);
+        p.down_items = p.down_tiles * row_groups * p.parts;
+        p.down_side = std::min(named(p.down_tile), std::max(1, 4096 / p.down_items));
+        launch_down(p, blocks_of(p.down_items, p.down_side), nt, s);
     }
     AF_TRY_LAUNCH();
 
@@ -942,17 +1012,17 @@ extern "C" int af_lora_add(const void* x, int64_t x_stride, int m, const int32_t
     p.slice_block[p.n_slices] = blocks;
     if (int64_t(blocks) * p.tiles > (1 << 22)) return AF_ERR_UNSUPPORTED;
     p.items = blocks * p.tiles;
-    dim3 up(unsigned(align_up(size_t(p.items), 8)));
     if (span) {
-        up.z = std::min(named(kTile) + (y != y_out), std::max(2, 2048 / p.items));
+        p.side = std::min(named(kTile) + (y != y_out), std::max(2, 2048 / p.items));
         if (y_dtype == AF_FP16)
-            launch_up_span<4, uint16_t>(p, up, s);
+            launch_up_span<4, uint16_t>(p, blocks_of(p.items, p.side), s);
         else
-            launch_up_span<2, float>(p, up, s);
+            launch_up_span<2, float>(p, blocks_of(p.items, p.side), s);
         AF_TRY_LAUNCH();
         return AF_OK;
     }
-    up.z = std::min(named(kTile) + (y != y_out), std::max(1, 4096 / p.items));
+    p.side = std::min(named(kTile) + (y != y_out), std::max(1, 4096 / p.items));
+    const dim3 up = blocks_of(p.items, p.side);
     if (y_dtype == AF_FP16) {
         if (mt == 4)
             launch_up<4, uint16_t>(p, up, s);
