@@ -64,7 +64,9 @@ __device__ __forceinline__ void store_fp8(uint8_t* p, const float (&v)[W]) {
                                                 true);
             w[i] = uint32_t(x);
         }
-        if constexpr (W == 8)
+        if constexpr (W == 16)
+            *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+        else if constexpr (W == 8)
             *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
         else
             *reinterpret_cast<uint32_t*>(p) = w[0];
@@ -79,7 +81,10 @@ __device__ __forceinline__ void load_fp8(const uint8_t* p, float (&v)[W]) {
     typedef float float2_t __attribute__((ext_vector_type(2)));
     if constexpr (W % 4 == 0) {
         uint32_t w[W / 4];
-        if constexpr (W == 8) {
+        if constexpr (W == 16) {
+            const uint4 u = *reinterpret_cast<const uint4*>(p);
+            w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+        } else if constexpr (W == 8) {
             const uint2 u = *reinterpret_cast<const uint2*>(p);
             w[0] = u.x, w[1] = u.y;
         } else {
