@@ -217,3 +217,63 @@ def test_plan_in_place_and_forked(gpu):
         now = got[:, :, np.array([ids[i // bs] * bs + i % bs for i in range(len(rows))], np.int64)]
         assert np.array_equal(now.view(np.uint16), logical[s][:, :, rows].view(np.uint16))
     bm.close()
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("layout", [AF_ROPE_HALF, AF_ROPE_INTERLEAVED])
+@pytest.mark.parametrize("layers,heads,hd,rot,bs", SHAPES)
+def test_new_blocks(gpu, fp8, layout, layers, heads, hd, rot, bs):
+    """Into blocks that nobody reads: all of them, or all but the first (then some rows move in place)."""
+    say(f"compact into new blocks fp8={fp8} layout={layout} {layers}x{heads}x{hd} rot={rot}")
+    if heads * hd * (1 if fp8 else 2) % 16:
+        pytest.skip("rows of whole 16 bytes")
+    r = np.random.default_rng(hd * 3 + bs)
+    lengths = [600, 2 * bs + 1, 350]
+    pages = max(-(-n // bs) for n in lengths)
+    pool = Pool(layers, 6 * pages, bs, heads, hd, fp8, hd)
+    ids = r.permutation(6 * pages).reshape(2, 3, pages).astype(np.int32)
+    src, dst = ids[0], ids[1].copy()
+    dst[2, 0] = src[2, 0]
+    keeps = [rows_of("half", n, r) for n in lengths]
+    cos, sin = table(600, rot)
+    launch(pool, src, dst, keeps, [0, 0, 0], rot, layout, cos, sin)
+    moves = [(src[i], dst[i], 0, keeps[i]) for i in range(3)]
+    assert_compact(pool.get(), pool.host, moves, bs, rot, layout, cos, sin)
+
+
+def test_bound_of_rows_far_above(gpu):
+    """max_rows is a bound: far above the sequences' rows, and below a workgroup's share of them."""
+    say("compact, max_rows of another order than the rows")
+    r = np.random.default_rng(6)
+    bs, n = 16, 900
+    cos, sin = table(n, 64)
+    for kind, most in (("window", 1 << 30), ("half", 1 << 30), ("window", 1 << 20)):
+        pool = Pool(1, 60, bs, 2, 64, False, 2)
+        tables = r.permutation(60)[None, :57].astype(np.int32)
+        keep = rows_of(kind, n, r)
+        f = 4 if kind == "window" else 0
+        launch(pool, tables, tables, [keep[f:]], [f], 64, 0, cos, sin, max_rows=most)
+        assert_compact(pool.get(), pool.host, [(tables[0], tables[0], f, keep[f:])], bs, 64, 0, cos, sin)
+
+
+def test_far_rows(gpu):
+    """Rows whose byte offsets pass 32 bits, of a layer whose slabs do too; in place, and in any order."""
+    say("compact, far rows")
+    bs, blocks, heads, hd = 16, 70000, 8, 128
+    row = heads * hd * 2
+    r = np.random.default_rng(1)
+    buf = dev.DeviceBuffer(2 * 2 * blocks * bs * row)
+    desc = kv.make_pool(buf.ptr, AF_KV_FP16, bs, 2, heads, hd, blocks)
+    table_ = np.array([[blocks - 1, 3, blocks - 2, 40000]], np.int32)
+    cos, sin = table(64, hd)
+    for keep in (np.arange(1, 60), np.arange(40, 62)):
+        data = r.standard_normal((2, 2, 64, heads, hd)).astype(np.float16)
+        at = lambda w, i: (w * blocks * bs + int(table_[0, i // bs]) * bs + i % bs) * row  # noqa: E731
+        for w in range(4):
+            for i in range(0, 64, bs):
+                buf.upload(data[w // 2, w % 2, i:i + bs], offset=at(w, i))
+        launch(type("P", (), {"desc": desc}), table_, table_, [keep], [0], hd, 0, cos, sin)
+        got = np.stack([np.stack([buf.download(np.float16, (bs, heads, hd), offset=at(w, i))
+                                  for i in range(0, 64, bs)]).reshape(64, heads, hd) for w in range(4)])
+        flat = np.arange(4, dtype=np.int32)
+        assert_compact(got.reshape(2, 2, 64, heads, hd), data, [(flat, flat, 0, keep)], bs, hd, 0, cos, sin)

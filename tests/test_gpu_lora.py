@@ -259,7 +259,8 @@ def test_lora_workspace_too_small(gpu):
 LARGE = [  # launches whose tiles fill the device: m, k, slice ends, max_rank, adapters
     (12300, 72, [130], 8, 5), (12289, 520, [33], 24, 3), (12290, 1288, [20, 41], 24, 6),
     (3100, 1304, [60, 120, 180, 215], 128, 3), (8300, 64, [2050, 4111], 16, 4), (4100, 64, [8200], 64, 3),
-    (2100, 64, [16400], 128, 5)]
+    (2100, 64, [16400], 128, 5), (2000, 4104, [40], 16, 12), (1500, 2056, [70, 100], 40, 5),
+    (900, 6152, [9, 18, 30], 64, 3)]
 
 
 @pytest.mark.parametrize("m,k,ends,rmax,count", LARGE)
