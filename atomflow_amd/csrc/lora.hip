@@ -978,30 +978,16 @@ extern "C" int af_lora_add(const void* x, int64_t x_stride, int m, const int32_t
 
     // the most adapters that n tokens in a row can name
     auto named = [&](int n) { return std::min(std::min(m, n), p.n_adapters); };
-    const int mt = m > 256 ? 4 : 1;
     hipStream_t s = static_cast<hipStream_t>(stream);
-
+    // Batches of up to 256 tokens are mostly decoded ones, few to an adapter; above, prompt chunks.
+    const bool chunks = m > 256;
     const int row_tiles = ceil_div(p.rows, 16);
     const int nt = std::min(4, row_tiles), row_groups = ceil_div(row_tiles, nt);
     p.tiles = ceil_div(m, kTile);
-    auto blocks_of = [](int items, int side) { return dim3(unsigned(align_up(size_t(items), 8)) * side); };
-    if (mt == 4 && p.tiles * row_groups * p.parts >= 192) {
-        p.splits = p.tiles * row_groups >= 192 ? 1 : p.parts;
-        p.down_tiles = p.tiles;
-        p.down_items = p.tiles * row_groups * p.splits;
-        p.down_side = std::min(named(kTile), std::max(2, 1024 / p.down_items));
-        launch_down_lds(p, blocks_of(p.down_items, p.down_side), nt, s);
-    } else {
-        p.splits = p.parts;
-        p.down_tile = mt == 4 ? 16 : kTile;
-        p.down_tiles = ceil_div(m, p.down_tile);
-        p.down_items = p.down_tiles * row_groups * p.parts;
-        p.down_side = std::min(named(p.down_tile), std::max(1, 4096 / p.down_items));
-        launch_down(p, blocks_of(p.down_items, p.down_side), nt, s);
-    }
-    AF_TRY_LAUNCH();
 
-    const bool span = mt == 4 && int64_t(p.tiles) * p.n >= int64_t(1024) * kSpan;
+    // `up` streams spans of columns where there are enough of them for every compute unit to have several
+    // (8192 tokens by 28672 columns: 222 us, by single blocks 260; 700 tokens: 25 and 24).
+    const bool span = chunks && int64_t(p.tiles) * p.n >= int64_t(1024) * kSpan;
     const int cols = span ? kSpan : kCols;
     int blocks = 0;
     for (int i = 0; i < p.n_slices; ++i) {
@@ -1012,6 +998,30 @@ extern "C" int af_lora_add(const void* x, int64_t x_stride, int m, const int32_t
     p.slice_block[p.n_slices] = blocks;
     if (int64_t(blocks) * p.tiles > (1 << 22)) return AF_ERR_UNSUPPORTED;
     p.items = blocks * p.tiles;
+    auto blocks_of = [](int items, int side) { return dim3(unsigned(align_up(size_t(items), 8)) * side); };
+
+    // The tiles' rows come through LDS where workgroups of 64 tokens and a part of K, or all of it, are
+    // enough for the device (2011 tokens, 14336 -> rank 16: 20 us, by registers 25; 3000 tokens, 4096 -> rank 16: 9
+    // and 11; 8192 tokens, 4096 -> twice rank 64: 46, by registers 84, with the parts left to `up` 61 and `up`
+    // 242 instead of 222). More workgroups to an item cost time where they find nothing to do, and save it
+    // where a tile names many adapters: 45 tokens of 24 adapters: `up` with 25 of them 17 us, with 9 12.5, with
+    // 4 15.5.
+    if (chunks && p.tiles * row_groups * p.parts >= 192) {
+        p.splits = p.tiles * row_groups >= 192 ? 1 : p.parts;
+        p.down_tiles = p.tiles;
+        p.down_items = p.tiles * row_groups * p.splits;
+        p.down_side = std::min(named(kTile), std::max(2, 1024 / p.down_items));
+        launch_down_lds(p, blocks_of(p.down_items, p.down_side), nt, s);
+    } else {
+        p.splits = p.parts;
+        p.down_tile = chunks ? 16 : kTile;
+        p.down_tiles = ceil_div(m, p.down_tile);
+        p.down_items = p.down_tiles * row_groups * p.parts;
+        p.down_side = std::min(named(p.down_tile), std::max(1, 768 / p.down_items));
+        launch_down(p, blocks_of(p.down_items, p.down_side), nt, s);
+    }
+    AF_TRY_LAUNCH();
+
     if (span) {
         p.side = std::min(named(kTile) + (y != y_out), std::max(2, 2048 / p.items));
         if (y_dtype == AF_FP16)
@@ -1021,15 +1031,15 @@ extern "C" int af_lora_add(const void* x, int64_t x_stride, int m, const int32_t
         AF_TRY_LAUNCH();
         return AF_OK;
     }
-    p.side = std::min(named(kTile) + (y != y_out), std::max(1, 4096 / p.items));
+    p.side = std::min(named(kTile) + (y != y_out), std::max(1, (chunks ? 2048 : 1024) / p.items));
     const dim3 up = blocks_of(p.items, p.side);
     if (y_dtype == AF_FP16) {
-        if (mt == 4)
+        if (chunks)
             launch_up<4, uint16_t>(p, up, s);
         else
             launch_up<1, uint16_t>(p, up, s);
     } else {
-        if (mt == 4)
+        if (chunks)
             launch_up<2, float>(p, up, s);
         else
             launch_up<1, float>(p, up, s);

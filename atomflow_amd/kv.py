@@ -54,11 +54,11 @@ def rope_frequencies(rot_dim, base=500000.0, scaling="none", factor=1.0, origina
         raise ValueError(f"scaling {scaling!r}: one of {', '.join(ROPE_SCALINGS)}")
     sc = _abi.RopeScaling(ROPE_SCALINGS[scaling], original_max_pos, base, factor, low_freq_factor,
                           high_freq_factor, beta_fast, beta_slow, attention_factor)
-    freq = np.empty(max(rot_dim, 0) // 2, np.float64)
+    freq = (ctypes.c_double * max(rot_dim // 2, 1))()
     mult = ctypes.c_double()
-    check(lib().af_rope_frequencies(ctypes.byref(sc), rot_dim, freq.ctypes.data,
-                                    ctypes.byref(mult)), "rope_frequencies")
-    return freq, mult.value
+    check(lib().af_rope_frequencies(ctypes.byref(sc), rot_dim, freq, ctypes.byref(mult)),
+          "rope_frequencies")
+    return np.frombuffer(freq, np.float64), mult.value
 
 
 def build_rope_table_scaled(d_cos, d_sin, first_pos, n_rows, rot_dim, freq, factor=1.0,
@@ -69,7 +69,7 @@ def build_rope_table_scaled(d_cos, d_sin, first_pos, n_rows, rot_dim, freq, fact
     if freq.shape != (rot_dim // 2,):
         raise ValueError(f"freq has shape {freq.shape}, rot_dim {rot_dim} needs ({rot_dim // 2},)")
     check(lib().af_rope_table_scaled(_p(d_cos), _p(d_sin), first_pos, n_rows, rot_dim,
-                                     freq.ctypes.data, factor, _s(stream)),
+                                     freq.__array_interface__["data"][0], factor, _s(stream)),
           "build_rope_table_scaled")
 
 
