@@ -240,17 +240,17 @@ __device__ __forceinline__ void few_tokens(const LoraArgs& p, const Adapters& to
     }
 }
 
-// Few tiles: a workgroup takes one part.
-template <int NT>
+// Few tiles: a workgroup takes one part and 16 rows (with 64 rows a workgroup, 2 tokens, 13952 -> twice rank 64
+// took 10.7 us instead of 5.4).
 __global__ __launch_bounds__(256) void lora_down_kernel(const LoraArgs p) {
-    __shared__ f32x4 sums[4][NT][64];
+    __shared__ f32x4 sums[4][1][64];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
     const Turn turn(p.down_items);
     const int item = 8 * turn.nth + turn.xcd;
     if (item >= p.down_items) return;
     const int t0 = item % p.down_tiles * p.down_tile, rest = item / p.down_tiles;
-    const int part = rest % p.parts, row0 = rest / p.parts * (16 * NT);
+    const int part = rest % p.parts, row0 = rest / p.parts * 16;
     int id = -1;
     if (lane < p.down_tile && t0 + lane < p.m) id = p.ids[t0 + lane];
     Adapters todo(id, id >= 0 && id < p.n_adapters);
@@ -260,7 +260,7 @@ __global__ __launch_bounds__(256) void lora_down_kernel(const LoraArgs p) {
         if (rank == 0) continue;
 #pragma unroll 1
         for (int base = 0; base < todo.count; base += 16)
-            few_tokens<NT>(p, todo, sums, t0, base, adapter, rank, row0, part, part + 1, part, lane, wave);
+            few_tokens<1>(p, todo, sums, t0, base, adapter, rank, row0, part, part + 1, part, lane, wave);
     }
 }
 
@@ -882,14 +882,6 @@ int lora_check(const af_lora* l) {
     return begin == l->n ? AF_OK : AF_ERR_INVALID_ARG;
 }
 
-void launch_down(const LoraArgs& p, dim3 grid, int nt, hipStream_t s) {
-    switch (nt) {
-        case 1: hipLaunchKernelGGL((lora_down_kernel<1>), grid, dim3(256), 0, s, p); break;
-        case 2: hipLaunchKernelGGL((lora_down_kernel<2>), grid, dim3(256), 0, s, p); break;
-        case 3: hipLaunchKernelGGL((lora_down_kernel<3>), grid, dim3(256), 0, s, p); break;
-        default: hipLaunchKernelGGL((lora_down_kernel<4>), grid, dim3(256), 0, s, p); break;
-    }
-}
 void launch_down_lds(const LoraArgs& p, dim3 grid, int nt, hipStream_t s) {
     switch (nt) {
         case 1: hipLaunchKernelGGL(lora_down_lds_kernel<1>, grid, dim3(256), 0, s, p); break;
@@ -1006,7 +998,7 @@ extern "C" int af_lora_add(const void* x, int64_t x_stride, int m, const int32_t
     // 242 instead of 222). More workgroups to an item cost time where they find nothing to do, and save it
     // where a tile names many adapters: 45 tokens of 24 adapters: `up` with 25 of them 17 us, with 9 12.5, with
     // 4 15.5.
-    if (chunks && p.tiles * row_groups * p.parts >= 192) {
+    if (chunks && p.tiles * row_groups * p.parts >= 96) {
         p.splits = p.tiles * row_groups >= 192 ? 1 : p.parts;
         p.down_tiles = p.tiles;
         p.down_items = p.tiles * row_groups * p.splits;
@@ -1016,9 +1008,9 @@ extern "C" int af_lora_add(const void* x, int64_t x_stride, int m, const int32_t
         p.splits = p.parts;
         p.down_tile = chunks ? 16 : kTile;
         p.down_tiles = ceil_div(m, p.down_tile);
-        p.down_items = p.down_tiles * row_groups * p.parts;
-        p.down_side = std::min(named(p.down_tile), std::max(1, 768 / p.down_items));
-        launch_down(p, blocks_of(p.down_items, p.down_side), nt, s);
+        p.down_items = p.down_tiles * row_tiles * p.parts;
+        p.down_side = std::min(named(p.down_tile), std::max(chunks ? 2 : 1, 1024 / p.down_items));
+        hipLaunchKernelGGL(lora_down_kernel, blocks_of(p.down_items, p.down_side), dim3(256), 0, s, p);
     }
     AF_TRY_LAUNCH();
 
