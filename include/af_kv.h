@@ -277,7 +277,7 @@ int af_rope_frequencies(const af_rope_scaling* scaling, int rot_dim, double* h_f
  * rows of rot_dim / 2 floats, the first at d_cos and d_sin (16-byte aligned).
  * h_freq is host memory and read before the call returns (a captured launch keeps the
  * values). Angles are reduced in 64 bits: each value is the exact one rounded to fp32
- * (off by no more than 0.51 steps of it, or 2^-50 n where the angle's n turns cost more).
+ * (off by no more than 0.51 steps of it, or 2^-51 of the angle where that is more).
  * The tables serve every entry point that takes cos_table and sin_table; those of the
  * unscaled form are af_rope_table_build's within its fp32 arithmetic. */
 int af_rope_table_scaled(float* d_cos, float* d_sin, int64_t first_pos, int n_rows, int rot_dim,
@@ -401,7 +401,8 @@ int af_kv_copy_blocks(const af_kv_pool* pool, const int32_t* d_copies, const int
  *   logical row f + i  <-  logical row d_keep[d_start[s] + i],   i = 0 .. n - 1,
  * through d_dst_tables[s] and d_src_tables[s] ([n_seqs][max_blocks] block ids each; the same
  * tables for a sequence that moves in place, other blocks where its own are shared:
- * af_bm_plan_compact makes both). d_keep is strictly increasing within a sequence, with
+ * af_bm_plan_compact makes both): a destination block is the source block of the same place, or one
+ * that nothing here reads. d_keep is strictly increasing within a sequence, with
  * d_keep[d_start[s] + i] >= f + i; then every row is read before it is written, whatever else
  * moves. No destination block is another sequence's source or destination.
  * rot_dim > 0: K is turned back by the rows' way up, from its position to its new one, in
