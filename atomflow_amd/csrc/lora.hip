@@ -18,9 +18,10 @@
 // Sums: K's parts and the order in which they are added are fixed by k alone, and every form adds
 // a token's products in the same order, so a token's row has the same bits whatever the launch.
 //
-// Measured (down + up): 1 token, 4096 -> 6144 columns in three slices, rank 16: 3.9 + 4.6 us, two chains of loads;
-// 45 tokens of 24 adapters, 4096 -> 28672, rank 32: 6.5 + 12.6 us (62 MB); 2011 tokens, 14336 -> 4096, rank 16: 18.5 + 18.4 us
-// (98 MB); 8192 tokens, 4096 -> 28672, rank 64: 48 + 225 us (y at 4.2 TB/s read and written).
+// Measured (down + up): 1 token, 4096 -> 6144 columns in three slices, rank 16: 3.9 + 4.6 us, two
+// chains of loads; 45 tokens of 24 adapters, 4096 -> 28672, rank 32: 6.5 + 12.6 us (62 MB); 2011
+// tokens, 14336 -> 4096, rank 16: 18.5 + 18.4 us (98 MB); 8192 tokens, 4096 -> 28672, rank 64:
+// 48 + 225 us (y at 4.2 TB/s read and written).
 #include <algorithm>
 #include <type_traits>
 
@@ -73,15 +74,6 @@ struct LoraArgs {
 
 __device__ __forceinline__ f16x8 load_f16x8(const uint16_t* p) {
     return __builtin_bit_cast(f16x8, *reinterpret_cast<const u32x4*>(p));
-}
-
-// Where `there` is false, any value: lanes that ask again for a line that is on its way wait for it one by
-// one, so what is not used is not loaded.
-__device__ __forceinline__ f16x8 load_f16x8_if(bool there, const uint16_t* p) {
-    f16x8 v;
-    v = __builtin_nondeterministic_value(v);
-    if (there) v = load_f16x8(p);
-    return v;
 }
 
 // The adapters that a tile's tokens name, in order of first appearance. Lane t holds token t's.
@@ -143,21 +135,18 @@ template <int MT, int NT>
 struct Operands {
     const uint16_t* x[MT];
     const uint16_t* a[NT];
-    bool x_on[MT], a_on[NT];  // (what a lane does not have touches its own sums alone, and those are not used)
     __device__ __forceinline__ Operands(const LoraArgs& p, const Adapters& some, int t0, int base, int adapter,
                                         int rank, int row0, int lane) {
         const int sub = 8 * (lane >> 4);
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            const int place = base + 16 * i + (lane & 15);
-            x[i] = p.x + size_t(t0 + some.token(place)) * p.x_stride + sub;
-            x_on[i] = place < some.count;
-        }
+        for (int i = 0; i < MT; ++i)
+            x[i] = p.x + size_t(t0 + some.token(base + 16 * i + (lane & 15))) * p.x_stride + sub;
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
             const int r = row0 + 16 * i + (lane & 15);
-            a_on[i] = r < p.rows && r % p.rmax < rank;
-            a[i] = p.a + (size_t(adapter) * p.rows + r) * p.k + sub;
+            const bool ok = r < p.rows && r % p.rmax < rank;
+            // (a row past the rank touches its own sums alone, and those are not used)
+            a[i] = p.a + (size_t(adapter) * p.rows + (ok ? r : row0)) * p.k + sub;
         }
     }
 };
@@ -204,9 +193,9 @@ __device__ __forceinline__ void few_tokens(const LoraArgs& p, const Adapters& to
         for (; k + 32 * kUnroll <= k1; k += 32 * kUnroll) {
 #pragma unroll
             for (int u = 0; u < kUnroll; ++u) {
-                xf[u][0] = load_f16x8_if(at.x_on[0], at.x[0] + k + 32 * u);
+                xf[u][0] = load_f16x8(at.x[0] + k + 32 * u);
 #pragma unroll
-                for (int i = 0; i < NT; ++i) af[u][i] = load_f16x8_if(at.a_on[i], at.a[i] + k + 32 * u);
+                for (int i = 0; i < NT; ++i) af[u][i] = load_f16x8(at.a[i] + k + 32 * u);
             }
 #pragma unroll
             for (int u = 0; u < kUnroll; ++u) multiply<1, NT>(xf, af, u, acc);
@@ -216,9 +205,9 @@ __device__ __forceinline__ void few_tokens(const LoraArgs& p, const Adapters& to
             for (int u = 0; u < kUnroll; ++u) {
                 const bool in = k + 32 * u + sub < k1;
                 if (k + 32 * u >= k1) break;
-                xf[u][0] = in && at.x_on[0] ? load_f16x8(at.x[0] + k + 32 * u) : f16x8{};
+                xf[u][0] = in ? load_f16x8(at.x[0] + k + 32 * u) : f16x8{};
 #pragma unroll
-                for (int i = 0; i < NT; ++i) af[u][i] = in && at.a_on[i] ? load_f16x8(at.a[i] + k + 32 * u) : f16x8{};
+                for (int i = 0; i < NT; ++i) af[u][i] = in ? load_f16x8(at.a[i] + k + 32 * u) : f16x8{};
             }
 #pragma unroll
             for (int u = 0; u < kUnroll; ++u) {
@@ -307,25 +296,20 @@ __global__ __launch_bounds__(256) void lora_down_lds_kernel(const LoraArgs p) {
         // Load j of a lane: row 8 j + lane / 8 of its 16 bytes; rows' 16 bytes are kept in the order
         // (piece ^ row) & 7, so that an operand's lanes read different banks.
         const int in_row = lane >> 3, piece = (lane & 7) ^ in_row;
-        // Rows that are not used stay as they are in LDS (they touch their own sums alone), but for one
-        // lane of each load, so that every load counts: lanes that ask for a line that others have asked
-        // for wait for it, one by one (a pass of 5 tokens with 59 copies took 60 us, without them 12).
         const uint16_t* from[kLoads];
         uint32_t to[kLoads];
-        bool on[kLoads];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const int r = 16 * wave + 8 * j + in_row;
             from[j] = p.x + size_t(t0 + todo.token(r)) * p.x_stride + k0 + 8 * piece;
             to[j] = lds0 + uint32_t(16 * wave + 8 * j) * 128;
-            on[j] = r < todo.count || lane == 0;
         }
 #pragma unroll
         for (int j = 0; j < kLoadsA; ++j) {
             const int first = 8 * ((wave + 4 * j) % (2 * NT));  // (two waves may load the same rows)
             const int r = row0 + first + in_row;
             const bool ok = r < p.rows && r % p.rmax < rank;
-            on[2 + j] = ok || lane == 0;
+            // (a row past the rank, or a place past the tokens, touches its own sums alone)
             from[2 + j] = p.a + (size_t(adapter) * p.rows + (ok ? r : row0)) * p.k + k0 + 8 * piece;
             to[2 + j] = lds0 + uint32_t(kTile + first) * 128;
         }
@@ -339,7 +323,7 @@ __global__ __launch_bounds__(256) void lora_down_lds_kernel(const LoraArgs p) {
             if (--ahead == 0) back = min(p.k - 8 - (k0 + 64 * (pieces - 1) + 8 * piece), 0);
 #pragma unroll
             for (int j = 0; j < kLoads; ++j) {
-                if (on[j]) lds_dma16(from[j] + back, to[j] + fill);
+                lds_dma16(from[j] + back, to[j] + fill);
                 from[j] += 64;
             }
             fill = fill == (kStages - 1) * kBytes ? 0 : fill + kBytes;
@@ -421,10 +405,6 @@ struct Run8;
 template <>
 struct Run8<uint16_t> {
     u32x4 w;
-    __device__ __forceinline__ void load_if(bool there, const uint16_t* p) {
-        w = __builtin_nondeterministic_value(w);
-        if (there) load(p);
-    }
     __device__ __forceinline__ void load(const uint16_t* p) { w = *reinterpret_cast<const u32x4_a2*>(p); }
     __device__ __forceinline__ void store(uint16_t* p) const { *reinterpret_cast<u32x4_a2*>(p) = w; }
     __device__ __forceinline__ void load_part(const uint16_t* p, int n) {
@@ -446,10 +426,6 @@ struct Run8<uint16_t> {
 template <>
 struct Run8<float> {
     f32x4 w[2];
-    __device__ __forceinline__ void load_if(bool there, const float* p) {
-        w[0] = w[1] = __builtin_nondeterministic_value(w[0]);
-        if (there) load(p);
-    }
     __device__ __forceinline__ void load(const float* p) {
         w[0] = *reinterpret_cast<const f32x4_a4*>(p);
         w[1] = *reinterpret_cast<const f32x4_a4*>(p + 4);
@@ -531,6 +507,7 @@ struct Columns {
     // From column c on, those below col1 (the others repeat the last one).
     __device__ __forceinline__ void load(const LoraArgs& p, int adapter, int c, int col1, int rank, int lane) {
         const int from = min(c, col1 - 1);
+        const int last = (rank - 1) & ~7;  // (ranks of the adapter alone are read)
         const uint16_t* at = p.b + (size_t(adapter) * p.n + from) * p.rmax;
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
@@ -539,7 +516,7 @@ struct Columns {
             const int off = min(col, col1 - 1 - from) * p.rmax;
 #pragma unroll
             for (int q = 0; q < KS; ++q)
-                f[t][q] = load_f16x8_if(32 * q + 8 * (lane >> 4) < rank, at + off + 32 * q + 8 * (lane >> 4));
+                f[t][q] = load_f16x8(at + off + min(32 * q + 8 * (lane >> 4), last));
         }
     }
     // What lies behind the adapter's rank is not used.
@@ -588,8 +565,8 @@ __device__ __forceinline__ void add_run(Run8<Y>& y, const f32x4 (&acc)[4], int h
     add_run(y, sum, up);
 }
 
-// Where a workgroup of `up` works: each XCD gets neighbouring items, which are the tiles by kGroup column blocks (whose part of B stays in its L2), then the next
-// column blocks.
+// Where a workgroup of `up` works: each XCD gets neighbouring items, which are the tiles by kGroup
+// column blocks (whose part of B stays in its L2), then the next column blocks.
 struct Place {
     bool any;
     int s, t0, col0, col1;
@@ -812,7 +789,8 @@ __global__ __launch_bounds__(256, KS == 1 ? 4 : KS == 2 ? 3 : 2) void lora_up_ke
         }
         Columns<KS> b;
         b.load(p, adapter, c, at.col1, rank, lane);
-        // Tokens from place `base` on, 16 to a tile.
+        // Tokens from place `base` on, 16 to a tile. (A place past the adapter's tokens reads the last
+        // one's y.)
         auto row = [&](int place, int64_t stride) {
             return size_t(at.t0 + todo.token(place)) * stride + c + 8 * (lane >> 4);
         };
@@ -822,9 +800,9 @@ __global__ __launch_bounds__(256, KS == 1 ? 4 : KS == 2 ? 3 : 2) void lora_up_ke
             for (int i = 0; i < MT; ++i) {
                 const int place = base + 16 * i + (lane & 15);
                 const Y* run = static_cast<const Y*>(p.y) + row(place, p.y_stride);
-                const bool there = whole && place < todo.count;
-                y[i][0].load_if(there, run);
-                y[i][1].load_if(there, run + 32);
+                run = whole ? run : reinterpret_cast<const Y*>(p.v);  // (anything that is there)
+                y[i][0].load(run);
+                y[i][1].load(run + 32);
             }
         };
         load_y(0);

@@ -583,9 +583,10 @@ size_t af_lora_workspace_size(const af_lora* lora, int m);
  *   y_out[i, j] = y[i, j] + scale * sum_r b[id, j, r] (sum_k a[id, s(j), r, k] x[i, k]),
  * id = d_ids[i], r < rank of id, s(j) the slice of column j. A token whose id is outside [0, n_adapters)
  * (-1: none), or whose adapter has rank 0, keeps y, bit for bit. Tokens of several adapters come in any order.
- * x rows x_stride elements apart (a multiple of 8, x 16-byte aligned); y and y_out rows of y_dtype (AF_FP16 or
- * AF_FP32), any alignment of their elements; y_out may be y (same stride), else they overlap nothing. fp32 sums, rounded once to
- * y_dtype. A token's row has the same bits whatever m and the other tokens are. m up to 2^20. */
+ * x rows x_stride elements apart (a multiple of 8, x 16-byte aligned); y and y_out rows of y_dtype
+ * (AF_FP16 or AF_FP32), any alignment of their elements; y_out may be y (same stride), else they
+ * overlap nothing. fp32 sums, rounded once to y_dtype. A token's row has the same bits whatever m
+ * and the other tokens are. m up to 2^20. */
 int af_lora_add(const void* x, int64_t x_stride, int m, const int32_t* d_ids, const af_lora* lora,
                 const void* y, int64_t y_stride, void* y_out, int64_t y_out_stride, int y_dtype,
                 void* workspace, size_t workspace_bytes, af_stream_t stream);
