@@ -953,9 +953,9 @@ extern "C" int af_lora_add(const void* x, int64_t x_stride, int m, const int32_t
     const int nt = std::min(4, row_tiles), row_groups = ceil_div(row_tiles, nt);
     p.tiles = ceil_div(m, kTile);
 
-    // `up` streams spans of columns where there are enough of them for every compute unit to have several
-    // (8192 tokens by 28672 columns: 222 us, by single blocks 260; 700 tokens: 25 and 24).
-    const bool span = chunks && int64_t(p.tiles) * p.n >= int64_t(1024) * kSpan;
+    // `up` streams spans of columns where there is one for every compute unit or so (8192 tokens by 28672
+    // columns: 222 us, by single blocks 278; 2000 tokens: 53 and 61; 3000 tokens by 4096 columns: 18 and 14).
+    const bool span = chunks && int64_t(p.tiles) * p.n >= int64_t(256) * kSpan;
     const int cols = span ? kSpan : kCols;
     int blocks = 0;
     for (int i = 0; i < p.n_slices; ++i) {
