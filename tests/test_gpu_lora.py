@@ -284,3 +284,49 @@ def test_lora_large(gpu, m, k, ends, rmax, count, y_dtype, pad, off):
     part.x, part.y, part.ids = (t[some].copy() for t in (c.x, c.y, c.ids))
     part.device().call()
     assert part.do.get().tobytes() == got[some].tobytes()
+
+
+@pytest.mark.parametrize("m,k,ends,rmax,count", [(2000, 4104, [40], 16, 12), (4100, 1032, [8200], 64, 3)])
+def test_lora_large_captured(gpu, m, k, ends, rmax, count):
+    """Prompt-sized launches replayed with other adapters, against eager launches of the same ids."""
+    say(f"lora large, captured m={m} k={k}")
+    st = dev.Stream()
+    c = Case(m, k, ends, rmax, count, 3).device()
+    c.call(stream=st)
+    st.sync()
+    g = dev.Graph.capture(st, lambda: c.call(stream=st))
+    r = np.random.default_rng(2)
+    for _ in range(3):
+        c.di.upload(np.repeat(r.integers(-1, count, m // 50 + 1), 50)[:m].astype(np.int32), st)
+        c.do.buf.fill_u32(0x5b5b5b5b, st)
+        c.ws.fill_u32(0x7fc00000, st)
+        g.launch(st)
+        st.sync()
+        got = c.do.get().tobytes()
+        c.call(stream=st)
+        st.sync()
+        assert c.do.get().tobytes() == got
+    g.destroy()
+    st.destroy()
+
+
+def test_lora_two_streams(gpu):
+    """Two projections' launches at once, each with its own workspace."""
+    say("lora, two streams")
+    cases = [Case(300, 2048, [700], 32, 9, 1).device(), Case(45, 4096, [512, 900], 16, 20, 2).device()]
+    want = []
+    for c in cases:
+        c.call()
+        want.append(c.do.get().tobytes())
+    streams = [dev.Stream(), dev.Stream()]
+    for _ in range(5):
+        for c, st in zip(cases, streams):
+            c.do.buf.fill_u32(0x5b5b5b5b, st)
+        for _ in range(4):
+            for c, st in zip(cases, streams):
+                c.call(stream=st)
+        for st in streams:
+            st.sync()
+        assert [c.do.get().tobytes() for c in cases] == want
+    for st in streams:
+        st.destroy()
