@@ -301,9 +301,9 @@ int launch_compact(CompactArgs& p, int n_seqs, int n_layers, hipStream_t s) {
     if (p.chunks > kThreads || n_layers > INT32_MAX / 2) return AF_ERR_UNSUPPORTED;
     p.groups = ceil_div(p.n_kv_heads, kHeadsInOrder);
     const int64_t others = int64_t(2) * n_layers * n_seqs;
-    // Long sequences, in order, where workgroups are few: longer steps (one sequence of 2000 rows, 28
-    // layers, half of them kept in place: 43 us, with 256 threads 59). Else 256 threads: 13 sequences of 3000 rows,
-    // 4 layers, FP8, into new blocks: 76 us, with 512 threads 82.
+    // Long sequences, in order, where workgroups are few: longer steps (one sequence of 2000 rows,
+    // 28 layers, half of them kept in place: 43 us, with 256 threads 59). Else 256 threads: 13
+    // sequences of 3000 rows, 4 layers, FP8, into new blocks: 76 us, with 512 threads 82.
     const int threads = p.chunks > 256 || (others * p.groups < 400 && p.max_rows > 512) ? 512 : 256;
     p.rows = threads / p.chunks;
     p.lanes = std::min(ceil_div(p.n_kv_heads, kHeadsOfThread), threads / p.chunks);

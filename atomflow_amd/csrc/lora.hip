@@ -111,12 +111,12 @@ __device__ __forceinline__ int rank_of(const LoraArgs& p, int adapter) {
     return p.ranks ? min(max(p.ranks[adapter], 0), p.rmax) : p.rmax;
 }
 
-// Workgroups go round the eight XCDs. An item has `side` of them, which share out its tile's adapters: first
-// every item's first one, then every item's second one, most of which find nothing to do. (Workgroups
-// start in order, dealt out to an XCD's shader engines in turn, and one that finds no room there keeps those
-// behind it waiting. Side by side instead, two to an item, all first ones fell on half of the engines, at
-// twice the time; and the order is one further in each round, so that a tile of many adapters has its
-// workgroups on different engines.)
+// Workgroups go round the eight XCDs. An item has `side` of them, which share out its tile's
+// adapters: first every item's first one, then every item's second one, most of which find nothing
+// to do. (Workgroups start in order, dealt out to an XCD's shader engines in turn, and one that
+// finds no room there keeps those behind it waiting. Side by side instead, two to an item, all
+// first ones fell on half of the engines, at twice the time; and the order is one further in each
+// round, so that a tile of many adapters has its workgroups on different engines.)
 struct Turn {
     int xcd, nth, skip;  // nth item of the XCD
     __device__ __forceinline__ explicit Turn(int items) {
@@ -173,8 +173,8 @@ __device__ __forceinline__ void store_v(const LoraArgs& p, const Adapters& some,
     }
 }
 
-// Up to 16 tokens of an adapter, from place `base` on, by all four waves: of each of the parts, a wave takes
-// one chain, kUnroll steps' loads before the first product; the four sums meet in LDS.
+// Up to 16 tokens of an adapter, from place `base` on, by all four waves: of each of the parts, a
+// wave takes one chain, kUnroll steps' loads before the first product; the four sums meet in LDS.
 template <int NT>
 __device__ __forceinline__ void few_tokens(const LoraArgs& p, const Adapters& todo, f32x4 (&sums)[4][NT][64], int t0,
                                            int base, int adapter, int rank, int row0, int part0, int part1,
@@ -233,8 +233,8 @@ __device__ __forceinline__ void few_tokens(const LoraArgs& p, const Adapters& to
     }
 }
 
-// Few tiles: a workgroup takes one part and 16 rows (with 64 rows a workgroup, 2 tokens, 13952 -> twice rank 64
-// took 10.7 us instead of 5.4).
+// Few tiles: a workgroup takes one part and 16 rows (with 64 rows a workgroup, 2 tokens, 13952 ->
+// twice rank 64 took 10.7 us instead of 5.4).
 __global__ __launch_bounds__(256) void lora_down_kernel(const LoraArgs p) {
     __shared__ f32x4 sums[4][1][64];
     const int lane = threadIdx.x & 63;
@@ -259,9 +259,9 @@ __global__ __launch_bounds__(256) void lora_down_kernel(const LoraArgs p) {
 
 // More tiles: 64 tokens by 16 NT rows, all waves on the same 64 of K at a time, which memory writes
 // straight to LDS (two pieces of 64 ahead), 8 lanes to the 128 bytes of a row. Neighbouring lanes
-// of a first or second operand are rows apart, so that loading operands from memory costs the address unit
-// 64 cycles an instruction; this way it is 16. A wave takes 16 of the tokens. With p.splits a workgroup takes
-// one part of K, else all of them.
+// of a first or second operand are rows apart, so that loading operands from memory costs the
+// address unit 64 cycles an instruction; this way it is 16. A wave takes 16 of the tokens. With
+// p.splits a workgroup takes one part of K, else all of them.
 template <int NT>
 __global__ __launch_bounds__(256) void lora_down_lds_kernel(const LoraArgs p) {
     constexpr int kRows = kTile + 16 * NT;       // LDS: the tokens' rows of x, then rows of A, of 128 bytes
@@ -293,8 +293,8 @@ __global__ __launch_bounds__(256) void lora_down_lds_kernel(const LoraArgs p) {
                            p.splits == 1 ? p.parts : part + 1, split, lane, wave);
             continue;
         }
-        // Load j of a lane: row 8 j + lane / 8 of its 16 bytes; rows' 16 bytes are kept in the order
-        // (piece ^ row) & 7, so that an operand's lanes read different banks.
+        // Load j of a lane: row 8 j + lane / 8 of its 16 bytes; rows' 16 bytes are kept in the
+        // order (piece ^ row) & 7, so that an operand's lanes read different banks.
         const int in_row = lane >> 3, piece = (lane & 7) ^ in_row;
         const uint16_t* from[kLoads];
         uint32_t to[kLoads];
@@ -399,7 +399,8 @@ __device__ __forceinline__ int scale_exponent(float top) {
 
 __device__ __forceinline__ float pow2f(int e) { return __builtin_ldexpf(1.0f, e); }
 
-// Eight neighbouring elements of y as they lie in memory; load_part and store_part: n of them, 1 .. 8.
+// Eight neighbouring elements of y as they lie in memory; load_part and store_part: n of them, 1 ..
+// 8.
 template <typename Y>
 struct Run8;
 template <>
@@ -498,9 +499,9 @@ struct Halves {
     }
 };
 
-// 64 columns of an adapter's B as four first operands: row 4 g + i of the t-th (g, i the result's lane
-// group and element) is column 32 (t / 2) + 8 g + 4 (t % 2) + i, so that a lane ends up with two runs
-// of 8 columns of one token, and a token's four lanes with 64 (fp16) bytes in a row.
+// 64 columns of an adapter's B as four first operands: row 4 g + i of the t-th (g, i the result's
+// lane group and element) is column 32 (t / 2) + 8 g + 4 (t % 2) + i, so that a lane ends up with
+// two runs of 8 columns of one token, and a token's four lanes with 64 (fp16) bytes in a row.
 template <int KS>
 struct Columns {
     f16x8 f[4][KS];
@@ -584,7 +585,8 @@ struct Place {
     }
 };
 
-// A tile's rows as they are (no adapter, or one of rank 0): columns [col0, col1) of its gathered tokens.
+// A tile's rows as they are (no adapter, or one of rank 0): columns [col0, col1) of its gathered
+// tokens.
 template <typename Y>
 __device__ __forceinline__ void copy_rows(const LoraArgs& p, const Adapters& some, int t0, int col0, int col1) {
     const int runs = (col1 - col0 + 7) / 8, total = some.count * runs;
@@ -647,10 +649,10 @@ __device__ __forceinline__ void last_columns(const LoraArgs& p, const Adapters& 
 
 // Many tiles: a tile's tokens of one adapter, gathered, by kSpan columns of one slice; rank up to
 // 32 KS. v is read and cut in halves once; then each wave takes 64 columns at a time, whose B and y
-// have been on their way since the 64 columns before. The products go through LDS, 16 tokens at a time, to
-// lanes that have y as it lies in memory: 8 lanes to the 64 columns of a token. (With a token's y in the
-// lanes that hold its products, neighbouring lanes are rows apart, and the address unit takes 64 cycles for
-// an instruction instead of 16.)
+// have been on their way since the 64 columns before. The products go through LDS, 16 tokens at a
+// time, to lanes that have y as it lies in memory: 8 lanes to the 64 columns of a token. (With a
+// token's y in the lanes that hold its products, neighbouring lanes are rows apart, and the address
+// unit takes 64 cycles for an instruction instead of 16.)
 template <int MT, int KS, typename Y>
 __global__ __launch_bounds__(256, 2) void lora_up_span_kernel(const LoraArgs p) {
     constexpr int kPer = Halves<KS>::kPer, kSlots = 256 / kPer;
@@ -758,9 +760,9 @@ __global__ __launch_bounds__(256, 2) void lora_up_span_kernel(const LoraArgs p) 
     }
 }
 
-// Fewer tiles: a tile's tokens of one adapter, gathered, by 256 columns of one slice, 64 to a wave. B
-// and y of the first 16 tokens are on their way while v is read and cut in halves. (64 tokens at a time
-// measured the same or, 2011 tokens by 4096 columns, 19 us instead of 17.)
+// Fewer tiles: a tile's tokens of one adapter, gathered, by 256 columns of one slice, 64 to a wave.
+// B and y of the first 16 tokens are on their way while v is read and cut in halves. (64 tokens at
+// a time measured the same or, 2011 tokens by 4096 columns, 19 us instead of 17.)
 template <int KS, typename Y>
 __global__ __launch_bounds__(256, KS == 1 ? 5 : KS == 2 ? 4 : 3) void lora_up_kernel(const LoraArgs p) {
     constexpr int kPer = Halves<KS>::kPer, kSlots = 256 / kPer;  // tokens whose v is read at a time
@@ -790,8 +792,8 @@ __global__ __launch_bounds__(256, KS == 1 ? 5 : KS == 2 ? 4 : 3) void lora_up_ke
         }
         Columns<KS> b;
         b.load(p, adapter, c, at.col1, rank, lane);
-        // Tokens from place `base` on, 16 to a tile. (A place past the adapter's tokens reads the last
-        // one's y.)
+        // Tokens from place `base` on, 16 to a tile. (A place past the adapter's tokens reads the
+        // last one's y.)
         auto row = [&](int place, int64_t stride) {
             return size_t(at.t0 + todo.token(place)) * stride + c + 8 * (lane >> 4);
         };
@@ -953,8 +955,9 @@ extern "C" int af_lora_add(const void* x, int64_t x_stride, int m, const int32_t
     const int nt = std::min(4, row_tiles), row_groups = ceil_div(row_tiles, nt);
     p.tiles = ceil_div(m, kTile);
 
-    // `up` streams spans of columns where there is one for every compute unit or so (8192 tokens by 28672
-    // columns: 222 us, by single blocks 278; 2000 tokens: 53 and 61; 3000 tokens by 4096 columns: 18 and 14).
+    // `up` streams spans of columns where there is one for every compute unit or so (8192 tokens by
+    // 28672 columns: 222 us, by single blocks 278; 2000 tokens: 53 and 61; 3000 tokens by 4096
+    // columns: 18 and 14).
     const bool span = chunks && int64_t(p.tiles) * p.n >= int64_t(256) * kSpan;
     const int cols = span ? kSpan : kCols;
     int blocks = 0;
@@ -968,12 +971,12 @@ extern "C" int af_lora_add(const void* x, int64_t x_stride, int m, const int32_t
     p.items = blocks * p.tiles;
     auto blocks_of = [](int items, int side) { return dim3(unsigned(align_up(size_t(items), 8)) * side); };
 
-    // The tiles' rows come through LDS where workgroups of 64 tokens and a part of K, or all of it, are
-    // enough for the device (2011 tokens, 14336 -> rank 16: 20 us, by registers 25; 3000 tokens, 4096 -> rank 16: 9
-    // and 11; 8192 tokens, 4096 -> twice rank 64: 46, by registers 84, with the parts left to `up` 61 and `up`
-    // 242 instead of 222). More workgroups to an item cost time where they find nothing to do, and save it
-    // where a tile names many adapters: 45 tokens of 24 adapters: `up` with 25 of them 17 us, with 9 12.5, with
-    // 4 15.5.
+    // The tiles' rows come through LDS where workgroups of 64 tokens and a part of K, or all of it,
+    // are enough for the device (2011 tokens, 14336 -> rank 16: 20 us, by registers 25; 3000
+    // tokens, 4096 -> rank 16: 9 and 11; 8192 tokens, 4096 -> twice rank 64: 46, by registers 84,
+    // with the parts left to `up` 61 and `up` 242 instead of 222). More workgroups to an item cost
+    // time where they find nothing to do, and save it where a tile names many adapters: 45 tokens
+    // of 24 adapters: `up` with 25 of them 17 us, with 9 12.5, with 4 15.5.
     if (chunks && p.tiles * row_groups * p.parts >= 96) {
         p.splits = p.tiles * row_groups >= 192 ? 1 : p.parts;
         p.down_tiles = p.tiles;
@@ -982,8 +985,9 @@ extern "C" int af_lora_add(const void* x, int64_t x_stride, int m, const int32_t
         launch_down_lds(p, blocks_of(p.down_items, p.down_side), nt, s);
     } else {
         p.splits = p.parts;
-        // Tiles of 16 tokens read an adapter's rows more often, but side by side: 62 tokens of one adapter, 11720 ->
-        // 2 x rank 16: 4.1 us, with 64 tokens to a tile 9.7; 246 of three, 4872 -> 2 x rank 64: 13 and 8.2.
+        // Tiles of 16 tokens read an adapter's rows more often, but side by side: 62 tokens of one
+        // adapter, 11720 -> 2 x rank 16: 4.1 us, with 64 tokens to a tile 9.7; 246 of three, 4872
+        // -> 2 x rank 64: 13 and 8.2.
         const bool few = int64_t(ceil_div(m, 16)) * row_tiles * p.parts * named(16) <= 256;
         p.down_tile = chunks || few ? 16 : kTile;
         p.down_tiles = ceil_div(m, p.down_tile);

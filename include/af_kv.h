@@ -300,11 +300,11 @@ int af_rope_rows(const void* q, int64_t q_stride, void* q_out, int64_t q_out_str
 /* af_paged_rope_append in these forms: of m rows qkv[i] = [Q | K | V], Q turned into q_out, K
  * turned and V as it is into row d_slots[i] of the pool's layer. qkv is only read (q_out may
  * be qkv itself, with its stride: then the Q part is turned in place and K and V left). Slot
- * -1: a row that is not cached (padding); another slot outside the pool, or a position outside
- * [0, max_pos) (whose Q is copied unturned), caches nothing either and stores AF_ERR_OUT_OF_RANGE into
- * *d_status (if given). The slots of one call are distinct. FP8 pools: K and V / scale,
- * clamped to +-448 and rounded once, from the fp32 value (af_paged_rope_append rounds K to
- * fp16 first); NaN stays NaN. */
+ * -1: a row that is not cached (padding); another slot outside the pool, or a position outside [0,
+ * max_pos) (whose Q is copied unturned), caches nothing either and stores AF_ERR_OUT_OF_RANGE into
+ * *d_status (if given). The slots of one call are distinct. FP8 pools: K and V / scale, clamped to
+ * +-448 and rounded once, from the fp32 value (af_paged_rope_append rounds K to fp16 first); NaN
+ * stays NaN. */
 int af_paged_rope_append_rows(const void* qkv, int64_t qkv_stride, int m, void* q_out,
                               int64_t q_out_stride, int n_q_heads, const af_kv_pool* pool,
                               int layer, const int64_t* d_slots, const int32_t* d_positions,
@@ -558,9 +558,9 @@ int af_w8a8_gemm_form(int m, int n, int k, int32_t* form);
  *   a  fp16 [n_adapters][n_slices][max_rank][k],  b  fp16 [n_adapters][n][max_rank],
  * 16-byte aligned. Slice s is the product's columns [slice_end[s-1], slice_end[s]) (a fused QKV or
  * gate and up weight has one low-rank pair per part; slice_end[n_slices-1] = n).
- * ranks: device int32 [n_adapters], an adapter's own rank (0 .. max_rank, clamped; NULL: max_rank for
- * all): what a and b hold behind it is not used. scales: device fp32 [n_adapters] or NULL
- * (1). max_rank: a multiple of 8, at most 128; k a multiple of 8. */
+ * ranks: device int32 [n_adapters], an adapter's own rank (0 .. max_rank, clamped; NULL: max_rank
+ * for all): what a and b hold behind it is not used. scales: device fp32 [n_adapters] or NULL (1).
+ * max_rank: a multiple of 8, at most 128; k a multiple of 8. */
 #define AF_LORA_MAX_SLICES 4
 typedef struct af_lora {
     const void* a;
@@ -581,8 +581,9 @@ size_t af_lora_workspace_size(const af_lora* lora, int m);
 /* Adds each token's adapter to a projection that the tokens share (af_w8a16_gemm_batched's,
  * af_w8a8_gemm's; x is that projection's fp16 input):
  *   y_out[i, j] = y[i, j] + scale * sum_r b[id, j, r] (sum_k a[id, s(j), r, k] x[i, k]),
- * id = d_ids[i], r < rank of id, s(j) the slice of column j. A token whose id is outside [0, n_adapters)
- * (-1: none), or whose adapter has rank 0, keeps y, bit for bit. Tokens of several adapters come in any order.
+ * id = d_ids[i], r < rank of id, s(j) the slice of column j. A token whose id is outside [0,
+ * n_adapters) (-1: none), or whose adapter has rank 0, keeps y, bit for bit. Tokens of several
+ * adapters come in any order.
  * x rows x_stride elements apart (a multiple of 8, x 16-byte aligned); y and y_out rows of y_dtype
  * (AF_FP16 or AF_FP32), any alignment of their elements; y_out may be y (same stride), else they
  * overlap nothing. fp32 sums, rounded once to y_dtype. A token's row has the same bits whatever m
@@ -780,16 +781,17 @@ int af_bm_plan_decode(af_block_manager* bm, const int32_t* seqs, int n, int64_t*
 int af_bm_hold_copy_source(af_block_manager* bm, int block_id);
 int af_bm_release_copy_sources(af_block_manager* bm);
 /* Cuts n sequences (none twice) to some of their rows: sequence i keeps its logical rows
- * keep[keep_start[i]] .. keep[keep_start[i + 1] - 1], strictly increasing and within its length, and
- * is that many tokens long afterwards (none: empty). Writes what af_kv_compact then reads, to host
- * arrays: src_tables and dst_tables [n][max_blocks] (unused entries 0), moved (the rows that move, at most
- * as many as keep has), start [n + 1], first [n], *max_rows (0: nothing to launch). Rows in front of
- * the first one dropped stay in place. A block that has other references, or is held as a copy's source,
- * is left as it is and replaced by a new one. The moves are launched before anything that writes to blocks
- * handed out later (a block freed here may be one of their sources), and after the copies that are planned
- * already. Not for sequences that a scheduler runs. On an error (AF_ERR_POOL_EXHAUSTED, AF_ERR_BAD_SEQUENCE,
- * AF_ERR_OUT_OF_RANGE: a row outside the sequence, or max_blocks below a sequence's blocks,
- * AF_ERR_INVALID_ARG) nothing changes. */
+ * keep[keep_start[i]] .. keep[keep_start[i + 1] - 1], strictly increasing and within its length,
+ * and is that many tokens long afterwards (none: empty). Writes what af_kv_compact then reads, to
+ * host arrays: src_tables and dst_tables [n][max_blocks] (unused entries 0), moved (the rows that
+ * move, at most as many as keep has), start [n + 1], first [n], *max_rows (0: nothing to launch).
+ * Rows in front of the first one dropped stay in place. A block that has other references, or is
+ * held as a copy's source, is left as it is and replaced by a new one. The moves are launched
+ * before anything that writes to blocks handed out later (a block freed here may be one of their
+ * sources), and after the copies that are planned already. Not for sequences that a scheduler
+ * runs. On an error (AF_ERR_POOL_EXHAUSTED, AF_ERR_BAD_SEQUENCE, AF_ERR_OUT_OF_RANGE: a row
+ * outside the sequence, or max_blocks below a sequence's blocks, AF_ERR_INVALID_ARG) nothing
+ * changes. */
 int af_bm_plan_compact(af_block_manager* bm, const int32_t* seqs, int n, const int32_t* keep,
                        const int32_t* keep_start, int32_t* src_tables, int32_t* dst_tables,
                        int max_blocks, int32_t* moved, int32_t* start, int32_t* first,
