@@ -952,7 +952,7 @@ extern "C" int af_lora_add(const void* x, int64_t x_stride, int m, const int32_t
     // Batches of up to 256 tokens are mostly decoded ones, few to an adapter; above, prompt chunks.
     const bool chunks = m > 256;
     const int row_tiles = ceil_div(p.rows, 16);
-    const int nt = std::min(4, row_tiles), row_groups = ceil_div(row_tiles, nt);
+    const int row_groups = ceil_div(row_tiles, 4), nt = ceil_div(row_tiles, row_groups);
     p.tiles = ceil_div(m, kTile);
 
     // `up` streams spans of columns where there is one for every compute unit or so (8192 tokens by
