@@ -27,6 +27,7 @@
 
 #include "af_common.h"
 #include "af_device.h"
+#include "af_lora_split.h"
 
 namespace af {
 namespace {
@@ -44,8 +45,7 @@ constexpr int kTile = 64;     // tokens of a tile: one to a lane
 constexpr int kCols = 256;    // `up`: columns of a workgroup, the gathering form's
 constexpr int kSpan = 1024;   // and the other one's
 constexpr int kGroup = 8;     // `up`: column blocks that a tile's workgroups take one after the other
-constexpr int kParts = 8;     // parts of K, at most
-constexpr int kPartMin = 512; // k of a part, at least
+constexpr int kParts = kLoraParts;
 
 struct LoraArgs {
     const uint16_t* x;
@@ -278,9 +278,8 @@ __global__ __launch_bounds__(256) void lora_down_lds_kernel(const LoraArgs p) {
     int id = -1;
     if (t0 + lane < p.m) id = p.ids[t0 + lane];
     Adapters todo(id, id >= 0 && id < p.n_adapters);
-    const int k0 = p.splits == 1 ? 0 : split * p.part_k;
-    const int k1 = min(p.splits == 1 ? p.k : k0 + p.part_k, p.k);
-    const int pieces = (k1 - k0 + 63) / 64;  // (none: a part behind K)
+    const LoraRange range = lora_range(p.k, p.part_k, p.splits, split);
+    const int k0 = range.k0, pieces = range.pieces;  // (one at least: no part is empty)
     const uint32_t lds0 = lds_address(stage);
 
     int adapter;
@@ -317,10 +316,9 @@ __global__ __launch_bounds__(256) void lora_down_lds_kernel(const LoraArgs p) {
         uint32_t fill = 0;  // the next load's place
         int ahead = pieces;  // loads to come
         auto load = [&] {
-            if (ahead == 0) return;
+            if (ahead <= 0) return;
             // (past K the loads repeat what is there)
-            int back = 0;
-            if (--ahead == 0) back = min(p.k - 8 - (k0 + 64 * (pieces - 1) + 8 * piece), 0);
+            const int back = --ahead == 0 ? lora_pull_back(p.k, range, piece) : 0;
 #pragma unroll
             for (int j = 0; j < kLoads; ++j) {
                 lds_dma16(from[j] + back, to[j] + fill);
@@ -384,6 +382,8 @@ __global__ __launch_bounds__(256) void lora_down_lds_kernel(const LoraArgs p) {
 #pragma unroll
         for (int j = 0; j < NT; ++j)
             store_v(p, todo, split, t0, 16 * wave + (lane & 15), row0 + 16 * j + 4 * (lane >> 4), rank, total[j]);
+        // The next adapter writes here. No load is on its way: each wave has awaited its last piece's
+        // (there is one), and stands behind every other wave's wait since that piece's barrier.
         __syncthreads();
     }
 }
@@ -844,8 +844,6 @@ __global__ __launch_bounds__(256, KS == 1 ? 5 : KS == 2 ? 4 : 3) void lora_up_ke
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 bool aligned_to(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 
-int parts_of(int k) { return std::min(kParts, ceil_div(k, kPartMin)); }
-
 int lora_check(const af_lora* l) {
     if (!l || l->n_adapters <= 0 || l->max_rank <= 0 || l->n_slices <= 0 || l->k <= 0 || l->n <= 0)
         return AF_ERR_INVALID_ARG;
@@ -896,7 +894,7 @@ using namespace af;
 
 extern "C" size_t af_lora_workspace_size(const af_lora* lora, int m) {
     if (lora_check(lora) || m < 0) return 0;
-    return align_up(size_t(parts_of(lora->k)) * size_t(m > 0 ? m : 1) * lora->n_slices *
+    return align_up(size_t(lora_split(lora->k).parts) * size_t(m > 0 ? m : 1) * lora->n_slices *
                         lora->max_rank * sizeof(float),
                     256);
 }
@@ -942,8 +940,9 @@ extern "C" int af_lora_add(const void* x, int64_t x_stride, int m, const int32_t
     p.y_out = y_out;
     p.y_out_stride = y_out_stride;
     p.v = static_cast<float*>(workspace);
-    p.parts = parts_of(p.k);
-    p.part_k = int(align_up(size_t(ceil_div(p.k, p.parts)), 256));
+    const LoraSplit split = lora_split(p.k);
+    p.parts = split.parts;
+    p.part_k = split.part_k;
     p.n_slices = lora->n_slices;
 
     // the most adapters that n tokens in a row can name
