@@ -42,7 +42,8 @@ constexpr int kMinSpan = 64;
 // Target tokens per split of batched launches (equal work per workgroup).
 constexpr int kBatchSpan = 512;
 
-inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
+// (a + b - 1 would pass INT32_MAX where a is a caller's bound near it)
+inline int ceil_div(int a, int b) { return a / b + (a % b > 0); }
 inline size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 
 // Split-K buffers of the decode-attention kernels. Layout of a workspace:

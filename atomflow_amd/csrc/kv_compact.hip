@@ -238,11 +238,12 @@ __global__ __launch_bounds__(kThreads) void kv_compact_kernel(const CompactArgs 
     const int head0 = int(blockIdx.z) * HO;
     const int lane_row = int(threadIdx.x) / p.chunks;
     const bool here = lane_row < p.rows;
-    const int steps = (n + p.rows - 1) / p.rows;
+    const int steps = (n - 1) / p.rows + 1;
     auto plan = [&](int step) {
-        const int t = threadIdx.x, i = step * p.rows + t;
+        const int t = threadIdx.x;
+        const int64_t i = int64_t(step) * p.rows + t;  // (steps past the last one are planned too)
         if (t < p.rows)
-            meta[step % 3][t] = i < n ? M::plan(p, seq, begin, first, i, which == 0 && blockIdx.z == 0)
+            meta[step % 3][t] = i < n ? M::plan(p, seq, begin, first, int(i), which == 0 && blockIdx.z == 0)
                                       : Meta{-1, 0, 0};
     };
     struct Held {
