@@ -42,6 +42,7 @@ void BlockManager::initialize(const PoolConfig& cfg, bool allocate_pool, void* p
     for (int i = 0; i < cfg.total_blocks; ++i) free_list_[size_t(i)] = cfg.total_blocks - 1 - i;
     tables_.clear();
     live_.clear();
+    scheduled_.clear();
     scales_ = scales;
     if (allocate_pool) {
         af_kv_pool d = pool_desc();
@@ -140,11 +141,16 @@ KVBlock BlockManager::block(int block_id, int layer) const {
 int BlockManager::create_sequence() {
     tables_.emplace_back();
     live_.push_back(1);
+    scheduled_.push_back(0);
     return int(tables_.size()) - 1;
 }
 
 bool BlockManager::has_sequence(int seq) const {
     return seq >= 0 && seq < int(tables_.size()) && live_[size_t(seq)];
+}
+
+void BlockManager::mark_scheduled(int seq) {
+    if (has_sequence(seq)) scheduled_[size_t(seq)] = 1;
 }
 
 int BlockManager::fork_sequence(int src) {
@@ -153,6 +159,7 @@ int BlockManager::fork_sequence(int src) {
     for (int b : copy.block_ids) ++ref_[size_t(b)];
     tables_.push_back(std::move(copy));
     live_.push_back(1);
+    scheduled_.push_back(0);
     return int(tables_.size()) - 1;
 }
 
@@ -293,7 +300,7 @@ int BlockManager::plan_compact(const int* seqs, int n, const int* keep, const in
     if (!out || n < 0 || (n > 0 && (!seqs || !keep_start || keep_start[0] < 0)))
         return AF_ERR_INVALID_ARG;
     for (int i = 0; i < n; ++i)
-        if (!has_sequence(seqs[i])) return AF_ERR_BAD_SEQUENCE;
+        if (!has_sequence(seqs[i]) || scheduled(seqs[i])) return AF_ERR_BAD_SEQUENCE;
     std::vector<int> sorted(seqs, seqs + n);
     std::sort(sorted.begin(), sorted.end());
     if (std::adjacent_find(sorted.begin(), sorted.end()) != sorted.end()) return AF_ERR_INVALID_ARG;

@@ -66,6 +66,7 @@ void Scheduler::maybe_cache(StepPlan* plan, Entry& e) {
     CachedPrefix c;
     c.key = e.req.prefix_key;
     c.seq = bm_.fork_sequence(e.seq);
+    bm_.mark_scheduled(c.seq);
     c.len = e.req.prefix_len;
     c.group = next_group_++;
     e.share_group = c.group;
@@ -243,6 +244,7 @@ int Scheduler::plan_step(StepPlan* plan) {
         } else {
             e.seq = bm_.create_sequence();
         }
+        bm_.mark_scheduled(e.seq);
         int first = 0;
         const int st = bm_.extend(e.seq, n, &first, &cow);
         if (st) return st;  // cannot happen: the blocks were counted above

@@ -788,10 +788,10 @@ int af_bm_release_copy_sources(af_block_manager* bm);
  * Rows in front of the first one dropped stay in place. A block that has other references, or is
  * held as a copy's source, is left as it is and replaced by a new one. The moves are launched
  * before anything that writes to blocks handed out later (a block freed here may be one of their
- * sources), and after the copies that are planned already. Not for sequences that a scheduler
- * runs. On an error (AF_ERR_POOL_EXHAUSTED, AF_ERR_BAD_SEQUENCE, AF_ERR_OUT_OF_RANGE: a row
- * outside the sequence, or max_blocks below a sequence's blocks, AF_ERR_INVALID_ARG) nothing
- * changes. */
+ * sources), and after the copies that are planned already. On an error (AF_ERR_POOL_EXHAUSTED,
+ * AF_ERR_BAD_SEQUENCE: unknown, or one that a scheduler runs or caches, which counts its tokens
+ * itself (a fork of it is not), AF_ERR_OUT_OF_RANGE: a row outside the sequence, or max_blocks
+ * below a sequence's blocks, AF_ERR_INVALID_ARG) nothing changes. */
 int af_bm_plan_compact(af_block_manager* bm, const int32_t* seqs, int n, const int32_t* keep,
                        const int32_t* keep_start, int32_t* src_tables, int32_t* dst_tables,
                        int max_blocks, int32_t* moved, int32_t* start, int32_t* first,

@@ -116,6 +116,9 @@ public:
     int fork_sequence(int src);  // id or AF_ERR_BAD_SEQUENCE
     int free_sequence(int seq);
     bool has_sequence(int seq) const;
+    // A Scheduler marks the sequences that it runs or caches, for as long as they live.
+    void mark_scheduled(int seq);
+    bool scheduled(int seq) const { return has_sequence(seq) && scheduled_[size_t(seq)]; }
     const PageTable& table(int seq) const;  // throws std::out_of_range
     int seq_len(int seq) const;             // tokens, or AF_ERR_BAD_SEQUENCE
     int64_t slot_of(int seq, int pos) const;
@@ -136,8 +139,8 @@ public:
     // with other references (or held as a copy's source) keeps its rows, and the sequence gets a
     // new one. AF_ERR_POOL_EXHAUSTED, _BAD_SEQUENCE, _OUT_OF_RANGE, _INVALID_ARG: nothing changed.
     // Blocks that become free are handed out again by later calls, so the moves are launched
-    // before anything that writes to blocks planned later. Sequences that a Scheduler runs are not
-    // for this call: it counts their tokens and shared rows itself.
+    // before anything that writes to blocks planned later. Sequences that a Scheduler runs or caches
+    // are refused (_BAD_SEQUENCE): it counts their tokens and shared rows itself. A fork of one is not.
     int plan_compact(const int* seqs, int n, const int* keep, const int* keep_start,
                      CompactPlan* out);
 
@@ -158,6 +161,7 @@ private:
     std::vector<int> holds_;      // held block ids, in the order taken
     std::vector<PageTable> tables_;
     std::vector<uint8_t> live_;
+    std::vector<uint8_t> scheduled_;
     void* pool_ = nullptr;
     const float* scales_ = nullptr;
     bool owns_pool_ = false;
