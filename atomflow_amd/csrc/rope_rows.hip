@@ -297,7 +297,7 @@ extern "C" int af_rope_frequencies(const af_rope_scaling* sc, int rot_dim, doubl
         };
         lo = std::max(std::floor(pair_of(sc->beta_fast)), 0.0);
         hi = std::min(std::ceil(pair_of(sc->beta_slow)), double(rot_dim - 1));
-        factor = 0.1 * std::log(sc->factor) + 1.0;
+        factor = 0.1 * std::log(std::max(sc->factor, 1.0)) + 1.0;
     }
     for (int i = 0; i < rot_dim / 2; ++i) {
         const double f = std::pow(base, -2.0 * i / rot_dim);

@@ -247,7 +247,7 @@ int af_paged_rope_append(void* qkv_out, int batch, const af_kv_pool* pool, int l
  *           pairs that turn beta_fast and beta_slow times within original_max_pos:
  *           lo = max(floor(d(beta_fast)), 0), hi = min(ceil(d(beta_slow)), rot_dim - 1),
  *           d(b) = rot_dim ln(original_max_pos / (2 pi b)) / (2 ln base), hi - lo at least 0.001;
- *           cos and sin are multiplied by 0.1 ln(factor) + 1.
+ *           cos and sin are multiplied by 0.1 ln(factor) + 1 (1 for a factor of 1 or less).
  * attention_factor, where it is not 0, replaces the kind's own factor on cos and sin (1 but
  * for YARN). */
 #define AF_ROPE_SCALE_NONE 0
