@@ -640,7 +640,11 @@ class BlockManager:
         n = len(seqs)
         if len(keeps) != n:
             raise ValueError(f"{n} sequences, {len(keeps)} lists of rows")
-        keeps = [np.asarray(k, np.int32).reshape(-1) for k in keeps]
+        keeps = [np.asarray(k).reshape(-1) for k in keeps]
+        if any(k.size and k.dtype.kind not in "iu" for k in keeps):
+            raise ValueError("rows to keep are whole numbers (of a mask: its np.nonzero)")
+        # (a row that 32 bits do not hold is outside every sequence, and stays so)
+        keeps = [k.astype(np.int64).clip(-1, 2 ** 31 - 1).astype(np.int32) for k in keeps]
         start = np.zeros(n + 1, np.int32)
         start[1:] = np.cumsum([len(k) for k in keeps])
         keep = np.ascontiguousarray(np.concatenate(keeps + [np.zeros(1, np.int32)]))
