@@ -275,9 +275,10 @@ int af_rope_frequencies(const af_rope_scaling* scaling, int rot_dim, double* h_f
 /* Rows [first_pos, first_pos + n_rows) of the table of positions, in one launch:
  *   d_cos[r, i] = cos((first_pos + r) h_freq[i]) * factor, d_sin likewise,
  * rows of rot_dim / 2 floats, the first at d_cos and d_sin (16-byte aligned).
- * h_freq is host memory and read before the call returns (a captured launch keeps the
- * values). Angles are reduced in 64 bits: each value is the exact one rounded to fp32
- * (off by no more than 0.51 steps of it, or 2^-51 of the angle where that is more).
+ * first_pos up to INT32_MAX, rot_dim up to 256. h_freq is host memory and read before the call
+ * returns (a captured launch keeps the values). Angles are reduced in 64 bits: each value is the
+ * exact one rounded to fp32 (off by no more than 0.51 steps of it, or 2^-51 of the angle where that
+ * is more).
  * The tables serve every entry point that takes cos_table and sin_table; those of the
  * unscaled form are af_rope_table_build's within its fp32 arithmetic. */
 int af_rope_table_scaled(float* d_cos, float* d_sin, int64_t first_pos, int n_rows, int rot_dim,
@@ -286,11 +287,13 @@ int af_rope_table_scaled(float* d_cos, float* d_sin, int64_t first_pos, int n_ro
 /* Rotary positions of m rows: q_out[i] = row q[i] turned by table row d_positions[i] (p0 + i
  * where d_positions is NULL), heads h at + h * head_dim, likewise k (k NULL or n_k_heads 0:
  * q alone). Outputs may be the inputs themselves (same pointer and stride), else they
- * overlap nothing. inverse = 1 turns back. Strides in elements, >= heads * head_dim;
+ * overlap nothing. inverse = 1 turns back (by minus the angle; a table's factor on cos and sin
+ * multiplies both ways). head_dim up to 512. Strides in elements, >= heads * head_dim;
  * fp16 rows of any alignment (16 bytes, with rot_dim a multiple of 16, run fastest). Arithmetic as
  * af_rope's: with AF_ROPE_HALF and rot_dim = head_dim the same bits. A row whose position is not
  * in [0, max_pos) is left (copied) unturned, and AF_ERR_OUT_OF_RANGE stored into *d_status
- * (if given). Tables: [max_pos, rot_dim / 2] fp32, 16-byte aligned. */
+ * (if given); p0 + m past max_pos is refused by the call. Tables: [max_pos, rot_dim / 2] fp32,
+ * 16-byte aligned. */
 int af_rope_rows(const void* q, int64_t q_stride, void* q_out, int64_t q_out_stride, int n_q_heads,
                  const void* k, int64_t k_stride, void* k_out, int64_t k_out_stride, int n_k_heads,
                  int m, int head_dim, int rot_dim, int layout, int inverse, const float* cos_table,
@@ -413,7 +416,7 @@ int af_kv_copy_blocks(const af_kv_pool* pool, const int32_t* d_copies, const int
  * A row whose source or destination lies past max_blocks * block_size, whose block id is outside
  * the pool, that would move down, or whose way up is not in the tables is left out, and
  * AF_ERR_OUT_OF_RANGE stored into *d_status (if given). max_rows: at least the longest
- * sequence's n (rows past it are left out, silently); it sizes the launch. */
+ * sequence's n (rows past it are left out, silently); it sizes the launch. n_seqs up to 65535. */
 int af_kv_compact(const af_kv_pool* pool, const int32_t* d_src_tables, const int32_t* d_dst_tables,
                   int max_blocks, int n_seqs, const int32_t* d_keep, const int32_t* d_start,
                   const int32_t* d_first, int max_rows, int rot_dim, int layout,
@@ -560,7 +563,8 @@ int af_w8a8_gemm_form(int m, int n, int k, int32_t* form);
  * gate and up weight has one low-rank pair per part; slice_end[n_slices-1] = n).
  * ranks: device int32 [n_adapters], an adapter's own rank (0 .. max_rank, clamped; NULL: max_rank
  * for all): what a and b hold behind it is not used. scales: device fp32 [n_adapters] or NULL (1).
- * max_rank: a multiple of 8, at most 128; k a multiple of 8. */
+ * max_rank: a multiple of 8, at most 128; k a multiple of 8. k and n up to 2^24, n_adapters up to
+ * 2^20 (AF_ERR_UNSUPPORTED above, as for max_rank and k). */
 #define AF_LORA_MAX_SLICES 4
 typedef struct af_lora {
     const void* a;
@@ -587,7 +591,9 @@ size_t af_lora_workspace_size(const af_lora* lora, int m);
  * x rows x_stride elements apart (a multiple of 8, x 16-byte aligned); y and y_out rows of y_dtype
  * (AF_FP16 or AF_FP32), any alignment of their elements; y_out may be y (same stride), else they
  * overlap nothing. fp32 sums, rounded once to y_dtype. A token's row has the same bits whatever m
- * and the other tokens are. m up to 2^20. */
+ * and the other tokens are; what is not finite in a token's x or y, or its adapter, stays in the
+ * rows that use it, as infinities or NaN. m up to 2^20, and m n up to about 2^38
+ * (AF_ERR_UNSUPPORTED above). */
 int af_lora_add(const void* x, int64_t x_stride, int m, const int32_t* d_ids, const af_lora* lora,
                 const void* y, int64_t y_stride, void* y_out, int64_t y_out_stride, int y_dtype,
                 void* workspace, size_t workspace_bytes, af_stream_t stream);
