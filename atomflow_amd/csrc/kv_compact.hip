@@ -16,9 +16,9 @@
 //     no source within the step (or before it) is overwritten unread.
 // No workspace, no copy to spare blocks, no order between workgroups.
 //
-// Bound by memory: one sequence of 8192 rows cut to 1028, 28 layers, fp16, in 53 us (206 MB read and
+// Bound by memory: one sequence of 8192 rows cut to 1028, 28 layers, fp16, in 52 us (206 MB read and
 // written, 3.9 TB/s); 13 sequences of 3000 cut to half, 4 layers, FP8, into new blocks 77 us (3.7
-// TB/s), in place 86. Runs of 8 instead of 16 bytes, 8 heads to a thread instead of 4, and 2 or 4
+// TB/s), in place 87. Runs of 8 instead of 16 bytes, 8 heads to a thread instead of 4, and 2 or 4
 // rows measured the same within 10 %.
 #include <algorithm>
 

@@ -18,10 +18,10 @@
 // Sums: K's parts and the order in which they are added are fixed by k alone, and every form adds
 // a token's products in the same order, so a token's row has the same bits whatever the launch.
 //
-// Measured (down + up): 1 token, 4096 -> 6144 columns in three slices, rank 16: 4.1 + 4.5 us, two
-// chains of loads; 45 tokens of 24 adapters, 4096 -> 28672, rank 32: 6.4 + 12.2 us (62 MB); 2011
-// tokens, 14336 -> 4096, rank 16: 18.5 + 16.5 us (98 MB); 8192 tokens, 4096 -> 28672, rank 64:
-// 45 + 221 us (y at 4.3 TB/s read and written).
+// Measured (down + up): 1 token, 4096 -> 6144 columns in three slices, rank 16: 4.0 + 4.6 us, two
+// chains of loads; 45 tokens of 24 adapters, 4096 -> 28672, rank 32: 6.8 + 12.9 us (62 MB); 2011
+// tokens, 14336 -> 4096, rank 16: 18.4 + 16.1 us (98 MB); 8192 tokens, 4096 -> 28672, rank 64:
+// 45 + 225 us (y at 4.2 TB/s read and written).
 #include <algorithm>
 #include <type_traits>
 

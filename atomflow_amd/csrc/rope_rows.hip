@@ -57,7 +57,7 @@ __device__ __forceinline__ void turned(double t, double& c, double& s) {
 
 // V neighbouring pairs per thread, of every `step`-th row: their turns stay in registers, and the
 // loop has no division (with one, and the turns in LDS, 40 us). About 30 64-bit operations a pair
-// hide behind its 8 bytes: bound by the writes, 131072 rows of 64 pairs in 15.3 us, 4.4 TB/s.
+// hide behind its 8 bytes: bound by the writes, 131072 rows of 64 pairs in 15.0 us, 4.5 TB/s.
 template <int V>
 __global__ __launch_bounds__(256) void rope_table_kernel(const TableArgs p) {
     const int chunks = p.pairs / V, rows = 256 / chunks;
@@ -123,7 +123,7 @@ struct RowsArgs {
 
 // Threads: row, head, chunk of 2 W elements (W pairs where they turn), the chunk fastest. A thread
 // keeps its row and chunk, so its cos and sin, and walks over heads: the table costs 512 bytes a
-// row instead of a head. Bound by memory: 8192 rows of 48 heads of 128 into an FP8 cache in 42.7
+// row instead of a head. Bound by memory: 8192 rows of 48 heads of 128 into an FP8 cache in 42.8
 // us, 4.4 TB/s read and written (a plain copy reaches 4.9); one row 2.7 us, the launch.
 template <int LAYOUT, int CACHE, int W>
 __global__ __launch_bounds__(256) void rope_rows_kernel(const RowsArgs a) {
